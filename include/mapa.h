@@ -35,7 +35,9 @@ typedef struct ihipStream_t* mapa_stream_t; /* == hipStream_t */
  * [w | w] (the conv's channels doubled), written by mapa_gemm's out_s3 / out_s3_relu when dtype is MAPA_F16, and
  * accepted as an output dtype by mapa_layernorm, mapa_bilinear_ac and mapa_split_rows.  A value outside binary16's
  * range (|v| > 65504, or not finite) sets MAPA_FAULT_F16_RANGE. */
-enum { MAPA_F32 = 0, MAPA_BF16 = 1, MAPA_BF16X3 = 2, MAPA_F16 = 3, MAPA_F16X2 = 4 };
+/* MAPA_FP8 / MAPA_I8: page types of a paged K/V cache only (mapa_kv_cache): e4m3 (largest 448) and two's-complement
+ * 8-bit codes with one power-of-two exponent byte per row. */
+enum { MAPA_F32 = 0, MAPA_BF16 = 1, MAPA_BF16X3 = 2, MAPA_F16 = 3, MAPA_F16X2 = 4, MAPA_FP8 = 5, MAPA_I8 = 6 };
 enum { MAPA_A_DENSE = 0, MAPA_A_CONV3X3 = 1 };
 enum { MAPA_OUT_ROWMAJOR = 0, MAPA_OUT_PIXSHUF = 1 };
 /* GELU is the exact-erf form (nn.GELU()), erf evaluated branch-free to within 1.2 ulp of fp32 erff (two minimax
@@ -75,7 +77,10 @@ int mapa_stream_check(mapa_stream_t stream, const char* what);
 /* MAPA_FAULT_F16_RANGE: a MAPA_F16 / MAPA_F16X2 producer met a value outside binary16's range (the TF32-equivalent
  * heads' operands); the outputs of that forward are not trustworthy: MapAnything.infer / forward re-run the call with
  * the fp32-exact split-precision heads (MapAnything._range_fallback) instead of returning them. */
-enum { MAPA_FAULT_LN_BARRIER = 1, MAPA_FAULT_F16_RANGE = 2 };
+/* MAPA_FAULT_KV_RANGE: a paged K/V cache call (mapa_kv_cache_write / _read, mapa_attention_paged) read a page number,
+ * length or row offset from device memory that lies outside what the host stated (mapa_kv_cache, mapa_kv_batch); the
+ * rows concerned are skipped or computed from a page inside the cache, never from memory outside it. */
+enum { MAPA_FAULT_LN_BARRIER = 1, MAPA_FAULT_F16_RANGE = 2, MAPA_FAULT_KV_RANGE = 4 };
 int mapa_fault_slot_create(uint32_t** host, uint32_t** dev);
 int mapa_fault_slot_destroy(uint32_t* host);
 int mapa_fault_publish(uint32_t* dev_slot, mapa_stream_t stream);
@@ -455,6 +460,108 @@ int mapa_view_rays(const float* K, const float* rays_in, const float* depth_z, i
  * (sn = 3*C, sh = 64) before the attention. */
 int mapa_rope2d(void* tokens, int dtype, int B, int H, int N, int D, int64_t sb, int64_t sh, int64_t sn,
                 const int64_t* positions, float base, float f0, mapa_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * Rotary positions with several axes (time, row, column, ...): the general form of mapa_rope2d, out of place or in
+ * place, forward and backward, one or two tensors (queries and keys) in one launch.
+ * Tensor i (i < 2, x[i] may be NULL): x[i] -> y[i] (equal pointers AND strides: in place), shape (batch, heads[i],
+ * tokens, head_dim), element strides (b, h, n), contiguous head dim.  section[a] pairs belong to axis a; with
+ * S = sum(section), 2 S <= head_dim, the dims from 2 S on are copied.  Pair i (axis a, its j-th pair) turns by
+ * positions[b][n][a] * freq[i] radians (the angle is reduced in 64 bits): u' = u cos - v sin, v' = v cos + u sin;
+ * inverse != 0 turns back, which is the backward pass.  Columns of (u, v):
+ *   MAPA_ROPE_AXIAL        axis a's block of 2 section[a] dims is [u | v] (RoPE-2D's layout)
+ *   MAPA_ROPE_HALF         u = i, v = S + i
+ *   MAPA_ROPE_INTERLEAVED  u = 2 i, v = 2 i + 1
+ * positions: int64 (MAPA_POS_I64) or fp32 (MAPA_POS_F32), element strides (b, n, a); fp32 arithmetic, one rounding. */
+enum { MAPA_ROPE_AXIAL = 0, MAPA_ROPE_HALF = 1, MAPA_ROPE_INTERLEAVED = 2 };
+enum { MAPA_POS_I64 = 0, MAPA_POS_F32 = 1 };
+#define MAPA_ROPE_MAX_AXES 4
+#define MAPA_ROPE_MAX_PAIRS 128
+typedef struct {
+  int dtype; /* MAPA_F32, MAPA_BF16 or MAPA_F16 */
+  int batch, tokens, head_dim;
+  const void* x[2];
+  void* y[2];
+  int heads[2];
+  int64_t x_bstride[2], x_hstride[2], x_nstride[2];
+  int64_t y_bstride[2], y_hstride[2], y_nstride[2];
+  const void* positions;
+  int pos_dtype;
+  int64_t pos_bstride, pos_nstride, pos_astride;
+  int axes;
+  int section[MAPA_ROPE_MAX_AXES];
+  int layout;
+  int inverse;
+  double freq[MAPA_ROPE_MAX_PAIRS];
+} mapa_rope_axes_desc;
+int mapa_rope_axes(const mapa_rope_axes_desc* d, mapa_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------------
+ * Paged K/V cache: the keys and values of running scenes kept between calls, in pages of page_size tokens.
+ * Pages k / v: [num_pages][heads][page_size][64] of dtype MAPA_BF16 / MAPA_F16 (k_exp / v_exp NULL), or MAPA_FP8 /
+ * MAPA_I8 codes with exponent bytes k_exp / v_exp [num_pages][heads][page_size]: value = code * 2^(byte - 127), byte
+ * the least with max|row| <= 448 (127) * 2^(byte - 127), taken of max(max|row|, 2^-100).  A power of two makes the scaling exact, so a
+ * value is rounded once, at the store (to nearest even).  A row with a value that is not finite is held as NaN.
+ * page_size: a power of two, 16 .. 1024.
+ * mapa_kv_batch: `seqs` sequences; token position p of sequence b lives in page table[b * table_stride + p /
+ * page_size], row p % page_size.  kv_lens[b]: tokens in the cache, the new ones included; the new tokens of sequence b
+ * are the packed rows cu_new[b] .. cu_new[b + 1] - 1 and hold its last positions.  Rows from cu_new[seqs] to
+ * new_rows - 1 are padding: not read, not written.  max_new / max_kv: host-known upper bounds of a sequence's new
+ * tokens / cached tokens.  All three arrays are int32 device memory; what they hold is checked on the device
+ * (MAPA_FAULT_KV_RANGE).
+ * mapa_kv_cache_write: new rows k, v (f32 / bf16 / f16; element strides of row and head, contiguous 64) into their
+ *   pages.  Two sequences must not share a page that the call writes.
+ * mapa_kv_cache_read: positions 0 .. cu_rows[b + 1] - cu_rows[b] - 1 of every sequence to the packed rows from
+ *   cu_rows[b] on (k_out, v_out [rows][heads][64] with element strides, f32 / bf16 / f16); positions past kv_lens[b]
+ *   read as zero, rows from cu_rows[seqs] on are left as they are. */
+typedef struct {
+  int dtype;
+  int heads, page_size, num_pages;
+  void* k;
+  void* v;
+  uint8_t* k_exp;
+  uint8_t* v_exp;
+} mapa_kv_cache;
+typedef struct {
+  int seqs, table_stride;
+  const int32_t* table;
+  const int32_t* kv_lens;
+  const int32_t* cu_new;
+  int new_rows, max_new, max_kv;
+} mapa_kv_batch;
+int mapa_kv_cache_write(const mapa_kv_cache* c, const mapa_kv_batch* b, const void* k, const void* v, int dtype,
+                        int64_t k_rstride, int64_t k_hstride, int64_t v_rstride, int64_t v_hstride,
+                        mapa_stream_t stream);
+int mapa_kv_cache_read(const mapa_kv_cache* c, const mapa_kv_batch* b, const int32_t* cu_rows, int rows, void* k_out,
+                       void* v_out, int dtype, int64_t k_rstride, int64_t k_hstride, int64_t v_rstride,
+                       int64_t v_hstride, mapa_stream_t stream);
+
+/* Attention of the batch's new tokens over their sequences' pages (head dim 64), the paged form of mapa_attention.
+ * q / o [new_rows][heads][64] bf16 or f16, element strides of row and head; `heads` is a multiple of the cache's heads
+ * (query head h reads K/V head h / (heads / cache heads)).  16-bit pages have q's type.
+ * A query at position p (of kv_lens[b]) sees keys below: kv_lens[b] (mask_block 0), or the end of p's block of
+ * mask_block positions, (p / mask_block + 1) * mask_block, where that is less (1: causal; tokens per view: every view
+ * sees itself and the earlier ones).  A query that sees nothing (more new tokens than cached ones) gets o = 0,
+ * lse = -inf.  A query's output depends on the keys and values it sees alone, whatever the hidden rows hold.
+ * lse (optional): [heads][new_rows] natural log, as mapa_attn_merge takes it.
+ * scale: softmax scale on q.k (0 = 1/8).  workspace (mapa_attention_paged_workspace_bytes, any contents, not shared
+ * with a call that may run at the same time): fp32 partials of the key ranges that are computed apart when there are
+ * few rows; without it every row's keys are walked by one workgroup. */
+typedef struct {
+  mapa_kv_cache cache;
+  mapa_kv_batch batch;
+  int dtype, heads;
+  const void* q;
+  void* o;
+  int64_t q_rstride, q_hstride, o_rstride, o_hstride;
+  float* lse;
+  float scale;
+  int mask_block;
+  void* workspace;
+  int64_t workspace_bytes;
+} mapa_attn_paged_desc;
+int mapa_attention_paged(const mapa_attn_paged_desc* d, mapa_stream_t stream);
+int64_t mapa_attention_paged_workspace_bytes(const mapa_attn_paged_desc* d);
 
 /* dst[i] += src[i] (n % 4 == 0) */
 int mapa_add_f32(float* dst, const float* src, int64_t n, mapa_stream_t stream);

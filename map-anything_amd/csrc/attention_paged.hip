@@ -1,0 +1,990 @@
+// Attention of new tokens over a paged K/V cache (mapa_attention_paged): head dim 64, grouped heads, bf16 / f16 queries
+// over 16-bit, e4m3 or int8 pages, full / causal / block-causal.
+//
+//   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp2(c s_ij - m_i),  s_ij = q_i . k_j,  c = scale log2(e),  j < limit(i)
+//
+// Rows are (new token, query head of the group) pairs, token-major, so that all query heads of a K/V head share its
+// tiles.  Q enters the MFMA as it is and c is applied to the fp32 scores: folding c into a 16-bit Q would round it once
+// more, which costs as much accuracy as the rounding of the output.  P is rounded to 16 bits as an MFMA operand, its
+// sum is not.  The sums' reference m_i is the row's first tile's maximum, moved only when a tile's sum passes 2^8.
+//
+//  * attn_paged_chunk: 4 waves x 32 rows over 64-key tiles (as mapa_attention): S^T = K Q^T on 32x32x16 MFMAs, so a
+//    lane owns a row and P feeds O^T = V^T P^T without leaving registers.  16-bit pages go to LDS by DMA, 8-bit pages
+//    through registers (decoded exactly: code times a power of two), into the same swizzled image.
+//  * attn_paged_step: few rows (single tokens): every wave walks its own 32-key tiles with 16x16x32 MFMAs, K from
+//    memory straight into operand registers, V through a wave-private LDS tile for its transpose; no barrier until the
+//    four waves are joined.
+//  * keys are cut into ranges of `chunk` when rows alone do not fill the chip; attn_paged_merge joins the fp32 partials
+//    in a fixed order.
+#include <algorithm>
+#include <type_traits>
+
+#include "paged.h"
+#include "index_math.h"
+
+namespace {
+using namespace mapa_paged;
+
+constexpr int NT = 256;
+constexpr int QB = 128;  // rows of a chunk workgroup
+constexpr int KT = 64;   // keys of a chunk tile
+constexpr int ST = 32;   // keys of a step tile
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float LN2 = 0.6931471805599453f;
+constexpr float REBASE_SUM = 256.f;
+
+struct PagedArgs {
+  const char* page[2];  // K, V
+  const uint8_t* exp[2];
+  const int32_t* table;
+  const int32_t* kv_lens;
+  const int32_t* cu;
+  const uint16_t* q;
+  uint16_t* o;
+  float* lse;
+  int64_t qr, qh, orr, oh;
+  float* part_o;    // [splits][new_rows * heads][64]
+  float* part_lse;  // [splits][new_rows * heads], log2 domain
+  unsigned* fault;
+  float c;  // scale * log2(e)
+  int seqs, table_stride, new_rows, max_new, cap, num_pages, psl;
+  int heads, kv_heads, group;
+  int block;    // mask_block
+  int splits, chunk;
+  int tiles;    // row tiles of the grid (upper bound)
+  int per_tile; // tokens of a row tile
+};
+
+typedef short s4v __attribute__((ext_vector_type(4)));
+typedef short s8v __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+
+__device__ __forceinline__ s4v tr_read(const char* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)(p));
+}
+
+// keys that a query at position pos sees
+__device__ __forceinline__ int key_limit(int pos, int len, int block) {
+  if (block == 0) return len;
+  if (pos < 0) return 0;
+  const int64_t end = ((int64_t)(pos / block) + 1) * block;
+  return end < len ? (int)end : len;
+}
+
+// New tokens of sequence b: its row interval, checked
+__device__ __forceinline__ int new_tokens(const PagedArgs& p, int c0, int c1) {
+  if (c0 < 0 || c1 < c0 || c1 > p.new_rows || c1 - c0 > p.max_new) {
+    kv_fault(p.fault);
+    return 0;
+  }
+  return c1 - c0;
+}
+
+// The wave's view of a sequence's page table: lane i holds the (checked) page of logical page w0 + i, so a page number
+// is a v_readlane away from being a scalar; a new window is fetched every 64 pages.
+struct PageWindow {
+  int w0, pages;
+};
+__device__ __forceinline__ int load_window(const PagedArgs& p, const int32_t* row, int w0, int pages, int lane) {
+  int v = 0;
+  if (w0 + lane < pages) v = checked_page(row[w0 + lane], p.num_pages, p.fault);
+  return v;
+}
+
+// 8 codes -> 8 operand words of the query's type, times the row's power of two (exact unless it leaves the type)
+template <bool F16, bool I8>
+__device__ __forceinline__ bf16x8 decode8(uint2 w, float s) {
+  const f32x4 a = decode4<I8>(w.x, s), b = decode4<I8>(w.y, s);
+  const uint4 u = {pack_lp2(F16, a[0], a[1]), pack_lp2(F16, a[2], a[3]), pack_lp2(F16, b[0], b[1]),
+                   pack_lp2(F16, b[2], b[3])};
+  return __builtin_bit_cast(bf16x8, u);
+}
+
+// whether any of 8 operand words is an infinity or a NaN
+template <bool F16>
+__device__ __forceinline__ bool any_special(bf16x8 v) {
+  constexpr uint32_t E = F16 ? 0x7c007c00u : 0x7f807f80u, LO = E & 0xffffu, HI = E & 0xffff0000u;
+  const uint4 u = __builtin_bit_cast(uint4, v);
+  bool r = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w;
+    r |= ((w & LO) == LO) | ((w & HI) == HI);
+  }
+  return r;
+}
+// element j of 8 operand words, the others zero
+__device__ __forceinline__ bf16x8 only(bf16x8 v, int j) {
+  const uint4 u = __builtin_bit_cast(uint4, v);
+  const uint32_t m = (j & 1) ? 0xffff0000u : 0xffffu;
+  const int w = j >> 1;
+  const uint4 r = {w == 0 ? u.x & m : 0u, w == 1 ? u.y & m : 0u, w == 2 ? u.z & m : 0u, w == 3 ? u.w & m : 0u};
+  return __builtin_bit_cast(bf16x8, r);
+}
+
+template <bool F16>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  return pack_lp2(F16, a, b);
+}
+
+// ------------------------------------------------------------------------------------------------ chunk
+// CK: 0 = 16-bit pages of the query's type, 1 = e4m3, 2 = int8
+template <bool F16, int CK>
+__global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
+  constexpr int TILE = KT * 128;  // 64 rows x 128 B
+  __shared__ __attribute__((aligned(1024))) char lds[2 * 2 * TILE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hl = lane >> 5, l32 = lane & 31;
+
+  // work: (K/V head, key range, row tile), row tiles innermost (they share K/V), the last ones (the longest key
+  // ranges under a causal mask) first
+  const int nblk = p.tiles * p.splits * p.kv_heads;
+  const int w = mapa_idx::xcd_remap(blockIdx.x, nblk);
+  int tile = w % p.tiles;
+  const int hs = w / p.tiles, split = hs % p.splits, hk = hs / p.splits;
+  tile = p.tiles - 1 - tile;
+
+  // row tile -> (sequence, tile in it): a wave-wide prefix sum over the sequences' tile counts, 64 at a time
+  int b = -1, nq = 0, c0 = 0;
+  {
+    int before = 0;
+#pragma unroll 1
+    for (int s0 = 0; s0 < p.seqs; s0 += 64) {
+      const int s = s0 + lane;
+      int q0 = 0, n = 0;
+      if (s < p.seqs) {
+        q0 = p.cu[s];
+        n = new_tokens(p, q0, p.cu[s + 1]);
+      }
+      int sum = (n + p.per_tile - 1) / p.per_tile;
+      const int own = sum;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(sum, o, 64);
+        if (lane >= o) sum += up;
+      }
+      const uint64_t past = __ballot(before + sum > tile);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        b = s0 + l;
+        nq = __builtin_amdgcn_readlane(n, l);
+        c0 = __builtin_amdgcn_readlane(q0, l);
+        tile -= before + __builtin_amdgcn_readlane(sum - own, l);
+        break;
+      }
+      before += __builtin_amdgcn_readlane(sum, 63);
+    }
+  }
+  if (b < 0) return;
+  const int len = __builtin_amdgcn_readfirstlane(checked_len(p.kv_lens[b], p.cap, p.fault));
+  const int t0 = tile * p.per_tile;                       // first token of the tile, in its sequence
+  const int rows = min(p.per_tile, nq - t0) * p.group;    // rows of the tile
+  const int pos0 = len - nq + t0;                         // position of the first token
+  const int lim_lo = key_limit(pos0, len, p.block);
+  const int lim_hi = key_limit(pos0 + (rows - 1) / p.group, len, p.block);
+  const int k_begin = split * p.chunk, k_end = min(k_begin + p.chunk, lim_hi);
+
+  // this lane's row
+  const int r = wave * 32 + l32;
+  const int rc = min(r, rows - 1);
+  const int rt = rc / p.group, rg = rc - rt * p.group;
+  const int tok = c0 + t0 + rt, head = hk * p.group + rg;
+  const int limit = key_limit(pos0 + rt, len, p.block);
+  const int64_t prow = ((int64_t)split * p.new_rows + tok) * p.heads + head;  // row of the partials
+  if (k_begin >= k_end) {  // no key of this range is seen by any row of the tile
+    if (p.splits > 1) {
+      if (r < rows && hl == 0) p.part_lse[prow] = -INFINITY;
+    } else if (r < rows) {
+      uint16_t* o = p.o + (int64_t)tok * p.orr + head * p.oh + hl * 32;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(o)[i] = uint4{0, 0, 0, 0};
+      if (p.lse && hl == 0) p.lse[(int64_t)head * p.new_rows + tok] = -INFINITY;
+    }
+    return;
+  }
+  const int kt0 = k_begin / KT, kt1 = (k_end + KT - 1) / KT;
+  const int kt_free = min(lim_lo, k_end) / KT;  // tiles below: every key seen by every row
+
+  // pages
+  const int32_t* trow = p.table + (int64_t)b * p.table_stride;
+  const int pages = (len + (1 << p.psl) - 1) >> p.psl;
+  const int pmask = (1 << p.psl) - 1;
+  const int64_t page_rows = (int64_t)p.kv_heads << p.psl, head_rows = (int64_t)hk << p.psl;
+  int w0 = k_begin >> p.psl;
+  int win = load_window(p, trow, w0, pages, lane);
+  // row of the cache (head hk) of a 16-row-aligned key; keys past the last page: the last page (their rows are masked)
+  auto cache_row = [&](int key) __attribute__((always_inline)) {
+    const int lp = min(key >> p.psl, pages - 1);
+    const int page = __builtin_amdgcn_readlane(win, lp - w0);
+    return (int64_t)page * page_rows + head_rows + (key & pmask);
+  };
+  auto need_window = [&](int key0) __attribute__((always_inline)) {  // pages of keys [key0, key0 + 64) in the window
+    const int last = min((key0 + KT - 1) >> p.psl, pages - 1);
+    if (last - w0 >= 64) {
+      w0 = key0 >> p.psl;
+      win = load_window(p, trow, w0, pages, lane);
+    }
+  };
+
+  const char* zero = reinterpret_cast<const char*>(g_mapa_zero_page);
+  // 16-bit pages: 16 pieces of 8 rows x 128 B (K: 0..7, V: 8..15), four per wave; the 16-B column is XOR-swizzled on
+  // the source so that the LDS image stays lane-linear
+  auto stage16 = [&](int slot, int kt) __attribute__((always_inline)) {
+    char* dst = lds + slot * 2 * TILE;
+    const int key0 = kt * KT;
+    need_window(key0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int k8 = (i * 4 + wave) * 8;  // first tile row of the piece (K and V alike)
+      const int row = k8 + (lane >> 3), pos = lane & 7;
+      const int kc = (pos ^ ((row >> 1) & 7)) * 16, vc = (pos ^ (((row >> 1) & 1) << 2)) * 16;
+      const int64_t at = cache_row(key0 + k8) * 128;
+      const bool in = key0 + row < len;
+      const char* ks = in ? p.page[0] + at + (lane >> 3) * 128 + kc : zero;
+      const char* vs = in ? p.page[1] + at + (lane >> 3) * 128 + vc : zero;
+      __builtin_amdgcn_global_load_lds(ks, (lds_ptr_t)(dst + k8 * 128), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(vs, (lds_ptr_t)(dst + TILE + k8 * 128), 16, 0, 0);
+    }
+  };
+  // 8-bit pages: thread -> tile row tid / 4, 16 codes; loaded one tile ahead, decoded after the tile's products
+  uint4 creg[2] = {};
+  uint32_t ereg[2] = {};
+  bool cin = false;
+  auto load8 = [&](int kt) __attribute__((always_inline)) {
+    const int key0 = kt * KT;
+    need_window(key0);
+    const int row = tid >> 2;
+    const int64_t at = cache_row(key0 + wave * 16) + (lane >> 2);
+    cin = key0 + row < len;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      creg[x] = *reinterpret_cast<const uint4*>(p.page[x] + at * 64 + (lane & 3) * 16);
+      ereg[x] = p.exp[x][at];
+    }
+  };
+  auto store8 = [&](int slot) __attribute__((always_inline)) {
+    char* dst = lds + slot * 2 * TILE;
+    const int row = tid >> 2, ch = (lane & 3) * 2;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const float s = exponent_value(ereg[x]);
+      bf16x8 lo = decode8<F16, CK == 2>(uint2{creg[x].x, creg[x].y}, s);
+      bf16x8 hi = decode8<F16, CK == 2>(uint2{creg[x].z, creg[x].w}, s);
+      if (!cin) lo = hi = bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      const int sw = x == 0 ? (row >> 1) & 7 : ((row >> 1) & 1) << 2;
+      *reinterpret_cast<bf16x8*>(dst + x * TILE + row * 128 + ((ch ^ sw) << 4)) = lo;
+      *reinterpret_cast<bf16x8*>(dst + x * TILE + row * 128 + (((ch + 1) ^ sw) << 4)) = hi;
+    }
+  };
+  if constexpr (CK == 0) stage16(0, kt0);
+  else load8(kt0);
+
+  bf16x8 qf[4];
+  {
+    const uint16_t* q = p.q + (int64_t)tok * p.qr + head * p.qh;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) qf[kk] = *reinterpret_cast<const bf16x8*>(q + kk * 16 + 8 * hl);
+  }
+  if constexpr (CK != 0) store8(0);
+
+  f32x16 o[2];
+#pragma unroll
+  for (int d = 0; d < 2; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+  float m_ref = 0.f, l_run = 0.f;
+  const float c = p.c;
+
+  // FIRST: the range's first tile (sets m_ref).  MASK: keys of the tile may be hidden from rows.  SLOT: LDS slot.
+  auto tile_step = [&](int kt, auto first_tag, auto mask_tag, auto slot_tag) __attribute__((always_inline)) {
+    constexpr bool FIRST = decltype(first_tag)::value;
+    constexpr bool MASK = decltype(mask_tag)::value;
+    constexpr int cur = decltype(slot_tag)::value;
+    const char* Ks = lds + cur * 2 * TILE;
+    const char* Vs = Ks + TILE;
+    bf16x8 kf[2][4];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const int row = kb * 32 + l32;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        kf[kb][kk] = *reinterpret_cast<const bf16x8*>(Ks + row * 128 + (((kk * 2 + hl) ^ ((row >> 1) & 7)) << 4));
+    }
+    f32x16 st[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st[kb][i] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk) st[kb] = mfma32x32x16<F16>(kf[kb][kk], qf[kk], st[kb]);
+    }
+    // V^T fragments (transposed LDS reads): every LDS read of the tile is issued before the next tile's DMA
+    bf16x8 vf[2][2][2];
+    {
+      const int i4 = lane & 15, q4 = i4 >> 2, p4 = i4 & 3, grp = (lane >> 4) & 1;
+#pragma unroll
+      for (int dt = 0; dt < 2; ++dt) {
+        const int cc = dt * 32 + 16 * grp + 4 * p4;
+        const int ch = cc >> 3, within = (cc & 7) * 2;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const int R0 = kb * 32 + 16 * s + 4 * hl + q4, R1 = R0 + 8;
+            const s4v lo = tr_read(Vs + R0 * 128 + ((ch ^ (((R0 >> 1) & 1) << 2)) << 4) + within);
+            const s4v hi = tr_read(Vs + R1 * 128 + ((ch ^ (((R1 >> 1) & 1) << 2)) << 4) + within);
+            vf[dt][kb][s] = s8v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          }
+      }
+    }
+    if (kt + 1 < kt1) {
+      if constexpr (CK == 0) stage16(cur ^ 1, kt + 1);
+      else load8(kt + 1);
+    }
+    if constexpr (MASK) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = kt * KT + kb * 32 + (i & 3) + 8 * (i >> 2) + 4 * hl;
+          st[kb][i] = key < limit ? st[kb][i] : -INFINITY;
+        }
+    }
+
+    bf16x8 pf[2][2];
+    float ls;
+    auto exp_pack = [&]() __attribute__((always_inline)) {
+      float a[4];
+      const float nm = -m_ref;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          uint32_t pk[4];
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[kb][8 * s + j], c, nm));
+            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[kb][8 * s + j + 1], c, nm));
+            a[j & 3] = (kb == 0 && s == 0 && j < 4) ? e0 : a[j & 3] + e0;
+            a[(j + 1) & 3] = (kb == 0 && s == 0 && j < 4) ? e1 : a[(j + 1) & 3] + e1;
+            pk[j / 2] = pack16<F16>(e0, e1);
+          }
+          pf[kb][s] = __builtin_bit_cast(bf16x8, uint4{pk[0], pk[1], pk[2], pk[3]});
+        }
+      ls = (a[0] + a[1]) + (a[2] + a[3]);
+    };
+    auto row_max = [&]() __attribute__((always_inline)) {
+      float mx = st[0][0];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[kb][i]);
+      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+      return fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * c;
+    };
+    if constexpr (FIRST) {
+      const float m = row_max();
+      m_ref = fmaxf(m, -1e38f);  // finite also for a row that sees none of the range
+      exp_pack();
+    } else {
+      exp_pack();
+      if (__builtin_expect(__any(!(ls <= REBASE_SUM)), 0)) {  // NaN rebases too
+        const float m = fmaxf(row_max(), m_ref);
+        const float alpha = __builtin_amdgcn_exp2f(m_ref - m);
+        m_ref = m;
+        l_run *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+        exp_pack();
+      }
+    }
+    l_run += ls;
+    bool special = false;
+    if constexpr (MASK) {  // an infinity or NaN in V: zero times it must not reach the rows that do not see its key
+#pragma unroll
+      for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) special |= any_special<F16>(vf[dt][kb][s]);
+      special = __any(special);
+    }
+    if (MASK && __builtin_expect(special, 0)) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll 1
+          for (int jj = 0; jj < 16; ++jj) {  // one key at a time, added where it is seen
+            const int j = jj & 7, h2 = jj >> 3;
+            const int key = kt * KT + kb * 32 + 16 * s + (j & 3) + 8 * (j >> 2) + 4 * h2;
+            const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+            const bf16x8 pk = hl == h2 ? only(pf[kb][s], j) : z;
+#pragma unroll
+            for (int dt = 0; dt < 2; ++dt) {
+              const bf16x8 vk = hl == h2 ? only(vf[dt][kb][s], j) : z;
+              f32x16 t;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) t[i] = 0.f;
+              t = mfma32x32x16<F16>(vk, pk, t);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o[dt][i] = key < limit ? o[dt][i] + t[i] : o[dt][i];
+            }
+          }
+    } else {
+#pragma unroll
+      for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) o[dt] = mfma32x32x16<F16>(vf[dt][kb][s], pf[kb][s], o[dt]);
+    }
+    if constexpr (CK != 0) {
+      if (kt + 1 < kt1) store8(cur ^ 1);
+    }
+    __syncthreads();
+  };
+
+  using T_ = std::integral_constant<bool, true>;
+  using F_ = std::integral_constant<bool, false>;
+  using S0 = std::integral_constant<int, 0>;
+  using S1 = std::integral_constant<int, 1>;
+  __syncthreads();
+  int kt = kt0;
+  if (kt < kt_free) tile_step(kt, T_(), F_(), S0());
+  else tile_step(kt, T_(), T_(), S0());
+  ++kt;
+#pragma unroll 1
+  for (; kt + 1 < kt_free; kt += 2) {
+    tile_step(kt, F_(), F_(), S1());
+    tile_step(kt + 1, F_(), F_(), S0());
+  }
+  // the rest: at most one more free tile, then the masked ones (an extra mask on a free tile changes nothing)
+#pragma unroll 1
+  for (; kt < kt1; kt += 2) {
+    tile_step(kt, F_(), T_(), S1());
+    if (kt + 1 < kt1) tile_step(kt + 1, F_(), T_(), S0());
+  }
+
+  const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
+  // a row that sees keys of the range has a sum of one at least, unless every score is -inf (then NaN, as the formula)
+  const bool seen = limit > k_begin;
+  const float inv = seen ? 1.f / l_tot : 0.f;
+  const float lse2 = !seen ? -INFINITY : l_tot > 0.f ? m_ref + __log2f(l_tot) : __builtin_nanf("");
+  if (!seen) {
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+  }
+  if (p.splits == 1) {
+    uint16_t* obase = p.o + (int64_t)tok * p.orr + head * p.oh;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int gp = 0; gp < 2; ++gp) {  // 16-B row segments out of the two half-lanes' 8-B pieces
+        uint32_t y[2], x[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          y[i] = pack16<F16>(o[dt][8 * gp + 2 * i] * inv, o[dt][8 * gp + 2 * i + 1] * inv);
+          x[i] = pack16<F16>(o[dt][8 * gp + 4 + 2 * i] * inv, o[dt][8 * gp + 4 + 2 * i + 1] * inv);
+          const auto sw = __builtin_amdgcn_permlane32_swap(y[i], x[i], false, false);
+          y[i] = sw[0];
+          x[i] = sw[1];
+        }
+        if (r < rows) *reinterpret_cast<uint4*>(obase + dt * 32 + 16 * gp + 8 * hl) = uint4{y[0], y[1], x[0], x[1]};
+      }
+    if (p.lse && r < rows && hl == 0) p.lse[(int64_t)head * p.new_rows + tok] = lse2 * LN2;
+  } else if (r < rows) {
+    float* po = p.part_o + prow * HD;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(po + dt * 32 + 8 * g + 4 * hl) =
+            f32x4{o[dt][4 * g] * inv, o[dt][4 * g + 1] * inv, o[dt][4 * g + 2] * inv, o[dt][4 * g + 3] * inv};
+    if (hl == 0) p.part_lse[prow] = lse2;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ step
+// RB blocks of 16 rows (new tokens x query heads of the group) per workgroup; each of the 4 waves walks every fourth
+// 32-key tile of the workgroup's key range.
+template <bool F16, int CK, int RB>
+__global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
+  constexpr int VT = ST * 128;  // V tile of a wave
+  constexpr int RS = RB * 16;   // rows
+  constexpr int JOIN = 4 * RS * HD * 4;
+  __shared__ __attribute__((aligned(1024))) char lds[JOIN > 4 * VT ? JOIN : 4 * VT];
+  __shared__ float join_m[4][RS], join_l[4][RS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, l16 = lane & 15;
+
+  // (sequence, key range, K/V head): the heads of a range innermost, so that one table row serves neighbours
+  const int hk = blockIdx.x % p.kv_heads, bs = blockIdx.x / p.kv_heads, split = bs % p.splits, b = bs / p.splits;
+  const int c0 = p.cu[b];
+  const int nq = new_tokens(p, c0, p.cu[b + 1]);
+  const int len = checked_len(p.kv_lens[b], p.cap, p.fault);
+  const int rows = nq * p.group;
+  if (rows == 0) return;
+  const int pos0 = len - nq;
+  const int lim_lo = key_limit(pos0, len, p.block), lim_hi = key_limit(len - 1, len, p.block);
+  const int k_begin = split * p.chunk, k_end = min(k_begin + p.chunk, lim_hi);
+
+  int limit[RB], tok[RB], head[RB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const int r = min(rb * 16 + l16, rows - 1);
+    const int rt = r / p.group;
+    tok[rb] = c0 + rt;
+    head[rb] = hk * p.group + r - rt * p.group;
+    limit[rb] = key_limit(pos0 + rt, len, p.block);
+  }
+  if (k_begin >= k_end) {  // uniform: the whole workgroup leaves
+    for (int i = tid; i < rows * 8; i += NT) {
+      const int r = i >> 3, rt = r / p.group, h = hk * p.group + r - rt * p.group, t = c0 + rt;
+      if (p.splits > 1) {
+        if ((i & 7) == 0) p.part_lse[((int64_t)split * p.new_rows + t) * p.heads + h] = -INFINITY;
+      } else {
+        reinterpret_cast<uint4*>(p.o + (int64_t)t * p.orr + h * p.oh)[i & 7] = uint4{0, 0, 0, 0};
+        if (p.lse && (i & 7) == 0) p.lse[(int64_t)h * p.new_rows + t] = -INFINITY;
+      }
+    }
+    return;
+  }
+
+  const int32_t* trow = p.table + (int64_t)b * p.table_stride;
+  const int pages = (len + (1 << p.psl) - 1) >> p.psl;
+  const int pmask = (1 << p.psl) - 1;
+  const int64_t page_rows = (int64_t)p.kv_heads << p.psl, head_rows = (int64_t)hk << p.psl;
+  int w0 = k_begin >> p.psl;
+  int win = load_window(p, trow, w0, pages, lane);
+  auto cache_row = [&](int key) __attribute__((always_inline)) {
+    const int lp = min(key >> p.psl, pages - 1);
+    const int page = __builtin_amdgcn_readlane(win, lp - w0);
+    return (int64_t)page * page_rows + head_rows + (key & pmask);
+  };
+
+  bf16x8 qf[RB][2];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const uint16_t* q = p.q + (int64_t)tok[rb] * p.qr + head[rb] * p.qh;
+    // 8-bit pages hand a lane 16 neighbouring dims of a key (one 16-B load): Q follows that order
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk)
+      qf[rb][kk] = *reinterpret_cast<const bf16x8*>(q + (CK == 0 ? kk * 32 + 8 * g : 16 * g + 8 * kk));
+  }
+
+  struct Tile {
+    uint4 k[CK == 0 ? 4 : 2];  // 16-bit: [key block][32 dims]; codes: [key block]
+    uint4 v[CK == 0 ? 4 : 2];  // 16-bit: rows 8 i + lane / 8; codes: rows 16 i + lane / 4
+    uint32_t ke[2], ve[2];
+  };
+  auto load = [&](Tile& t, int key0) __attribute__((always_inline)) {
+    const int last = min((key0 + ST - 1) >> p.psl, pages - 1);
+    if (last - w0 >= 64) {
+      w0 = key0 >> p.psl;
+      win = load_window(p, trow, w0, pages, lane);
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const int64_t at = cache_row(key0 + 16 * kb);
+      if constexpr (CK == 0) {
+        const char* kp = p.page[0] + (at + l16) * 128 + g * 16;
+        t.k[2 * kb] = *reinterpret_cast<const uint4*>(kp);
+        t.k[2 * kb + 1] = *reinterpret_cast<const uint4*>(kp + 64);
+        const char* vp = p.page[1] + (at + (lane >> 3)) * 128 + (lane & 7) * 16;
+        t.v[2 * kb] = *reinterpret_cast<const uint4*>(vp);
+        t.v[2 * kb + 1] = *reinterpret_cast<const uint4*>(vp + 8 * 128);
+      } else {
+        t.k[kb] = *reinterpret_cast<const uint4*>(p.page[0] + (at + l16) * 64 + g * 16);
+        t.ke[kb] = p.exp[0][at + l16];
+        t.v[kb] = *reinterpret_cast<const uint4*>(p.page[1] + (at + (lane >> 2)) * 64 + (lane & 3) * 16);
+        t.ve[kb] = p.exp[1][at + (lane >> 2)];
+      }
+    }
+  };
+
+  f32x4 o[RB][4];
+  float m_ref[RB], l_run[RB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    m_ref[rb] = -INFINITY;
+    l_run[rb] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) o[rb][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const float c = p.c;
+  char* Vs = lds + wave * VT;
+  // V's 16-B column is XOR-swizzled by its row, so that the transposed reads of four rows hit different banks
+  auto vslot = [&](int row, int ch) __attribute__((always_inline)) { return Vs + row * 128 + ((ch ^ ((row & 3) << 1)) << 4); };
+
+  auto tile_step = [&](const Tile& t, int key0) __attribute__((always_inline)) {
+    const bool mask = key0 + ST > lim_lo;
+    // V to LDS (rows past the sequence as zeros: whatever their memory holds must not meet a zero weight)
+#pragma unroll
+    for (int i = 0; i < (CK == 0 ? 4 : 2); ++i) {
+      if constexpr (CK == 0) {
+        const int row = 8 * i + (lane >> 3);
+        uint4 v = t.v[i];
+        if (mask && key0 + row >= len) v = uint4{0, 0, 0, 0};
+        *reinterpret_cast<uint4*>(vslot(row, lane & 7)) = v;
+      } else {
+        const int row = 16 * i + (lane >> 2);
+        const float s = exponent_value(t.ve[i]);
+        bf16x8 lo = decode8<F16, CK == 2>(uint2{t.v[i].x, t.v[i].y}, s);
+        bf16x8 hi = decode8<F16, CK == 2>(uint2{t.v[i].z, t.v[i].w}, s);
+        if (mask && key0 + row >= len) lo = hi = bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
+        *reinterpret_cast<bf16x8*>(vslot(row, (lane & 3) * 2)) = lo;
+        *reinterpret_cast<bf16x8*>(vslot(row, (lane & 3) * 2 + 1)) = hi;
+      }
+    }
+    bf16x8 kf[2][2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      if constexpr (CK == 0) {
+        kf[kb][0] = __builtin_bit_cast(bf16x8, t.k[2 * kb]);
+        kf[kb][1] = __builtin_bit_cast(bf16x8, t.k[2 * kb + 1]);
+      } else {
+        const float s = exponent_value(t.ke[kb]);
+        kf[kb][0] = decode8<F16, CK == 2>(uint2{t.k[kb].x, t.k[kb].y}, s);
+        kf[kb][1] = decode8<F16, CK == 2>(uint2{t.k[kb].z, t.k[kb].w}, s);
+      }
+    }
+    // V^T fragments: dims 16 dt + l16, keys 4 g .. + 3 and 16 + 4 g .. + 3 (the order the scores come in)
+    bf16x8 vf[4];
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt) {
+      const int q4 = l16 >> 2, p4 = l16 & 3;
+      const int row = 4 * g + q4, ch = dt * 2 + (p4 >> 1), within = (p4 & 1) * 8;
+      const s4v lo = tr_read(vslot(row, ch) + within);
+      const s4v hi = tr_read(vslot(row + 16, ch) + within);
+      vf[dt] = s8v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    }
+    bool special = false;
+    if (mask) {
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) special |= any_special<F16>(vf[dt]);
+      special = __any(special);
+    }
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      f32x4 st[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        st[kb] = mfma16x16x32<F16>(kf[kb][0], qf[rb][0], f32x4{0.f, 0.f, 0.f, 0.f});
+        st[kb] = mfma16x16x32<F16>(kf[kb][1], qf[rb][1], st[kb]);
+      }
+      if (mask) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) st[kb][i] = key0 + 16 * kb + 4 * g + i < limit[rb] ? st[kb][i] : -INFINITY;
+      }
+      float mx = fmaxf(fmaxf(fmaxf(st[0][0], st[0][1]), fmaxf(st[0][2], st[0][3])),
+                       fmaxf(fmaxf(st[1][0], st[1][1]), fmaxf(st[1][2], st[1][3])));
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
+      const float m_new = fmaxf(m_ref[rb], mx);
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;  // nothing seen yet
+      const float alpha = __builtin_amdgcn_exp2f(m_ref[rb] - m_use);
+      m_ref[rb] = m_new;
+      float e[8], ls = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i >> 2][i & 3], c, -m_use));
+        ls += e[i];
+      }
+      l_run[rb] = l_run[rb] * alpha + ls;
+      const bf16x8 pf = __builtin_bit_cast(bf16x8, uint4{pack16<F16>(e[0], e[1]), pack16<F16>(e[2], e[3]),
+                                                         pack16<F16>(e[4], e[5]), pack16<F16>(e[6], e[7])});
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) o[rb][dt] *= alpha;
+      if (__builtin_expect(special, 0)) {
+#pragma unroll 1
+        for (int jj = 0; jj < 32; ++jj) {  // one key at a time, added where it is seen
+          const int j = jj & 7, g2 = jj >> 3;
+          const int key = key0 + 4 * g2 + (j & 3) + 16 * (j >> 2);
+          const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+          const bf16x8 pk = g == g2 ? only(pf, j) : z;
+#pragma unroll
+          for (int dt = 0; dt < 4; ++dt) {
+            const bf16x8 vk = g == g2 ? only(vf[dt], j) : z;
+            const f32x4 x = mfma16x16x32<F16>(vk, pk, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[rb][dt][i] = key < limit[rb] ? o[rb][dt][i] + x[i] : o[rb][dt][i];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) o[rb][dt] = mfma16x16x32<F16>(vf[dt], pf, o[rb][dt]);
+      }
+    }
+  };
+
+  // two tiles in registers: the loads of one fly while the other is used
+  constexpr int STEP = 4 * ST;
+  Tile ta, tb;
+  int key = k_begin + wave * ST;
+  if (key < k_end) load(ta, key);
+  if (key + STEP < k_end) load(tb, key + STEP);
+#pragma unroll 1
+  while (key < k_end) {
+    tile_step(ta, key);
+    if (key + 2 * STEP < k_end) load(ta, key + 2 * STEP);
+    key += STEP;
+    if (key >= k_end) break;
+    tile_step(tb, key);
+    if (key + 2 * STEP < k_end) load(tb, key + 2 * STEP);
+    key += STEP;
+  }
+
+  // join the four waves: fp32 rows, maxima and sums through LDS
+  __syncthreads();
+  float* jo = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    float l = l_run[rb];
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    const int row = rb * 16 + l16;
+    if (g == 0) {
+      join_m[wave][row] = m_ref[rb];
+      join_l[wave][row] = l;
+    }
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+      *reinterpret_cast<f32x4*>(jo + (wave * RS + row) * HD + dt * 16 + 4 * g) = o[rb][dt];
+  }
+  __syncthreads();
+  for (int i = tid; i < rows * 16 && i < RS * 16; i += NT) {
+    const int row = i >> 4, d = (i & 15) * 4;
+    const int rt = row / p.group, h = hk * p.group + row - rt * p.group, t = c0 + rt;
+    float m = join_m[0][row];
+#pragma unroll
+    for (int x = 1; x < 4; ++x) m = fmaxf(m, join_m[x][row]);
+    const bool seen = key_limit(pos0 + rt, len, p.block) > k_begin;
+    const float m_use = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float wgt = __builtin_amdgcn_exp2f(join_m[x][row] - m_use);
+      l += wgt * join_l[x][row];
+      acc += wgt * *reinterpret_cast<const f32x4*>(jo + (x * RS + row) * HD + d);
+    }
+    const float inv = 1.f / l;
+    const float lse2 = !seen ? -INFINITY : l > 0.f ? m_use + __log2f(l) : __builtin_nanf("");
+    f32x4 v = acc * inv;
+    if (!seen) v = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (p.splits == 1) {
+      *reinterpret_cast<uint2*>(p.o + (int64_t)t * p.orr + h * p.oh + d) =
+          uint2{pack16<F16>(v[0], v[1]), pack16<F16>(v[2], v[3])};
+      if (p.lse && d == 0) p.lse[(int64_t)h * p.new_rows + t] = lse2 * LN2;
+    } else {
+      const int64_t pr = ((int64_t)split * p.new_rows + t) * p.heads + h;
+      *reinterpret_cast<f32x4*>(p.part_o + pr * HD + d) = v;
+      if (d == 0) p.part_lse[pr] = lse2;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ merge
+// 16 lanes x 4 columns per row, MG groups of them over every MG-th key range, joined by a fixed butterfly.
+template <bool F16, int MG>
+__global__ void __launch_bounds__(NT) attn_paged_merge(PagedArgs p) {
+  const int64_t total = (int64_t)p.new_rows * p.heads;
+  const int64_t e = (int64_t)blockIdx.x * (NT / (16 * MG)) + threadIdx.x / (16 * MG);
+  const int64_t row = e < total ? e : total - 1;
+  const int d = (threadIdx.x & 15) * 4, mg = (threadIdx.x >> 4) % MG;
+  const int t = (int)(row / p.heads), h = (int)(row % p.heads);
+  const bool live = e < total && t >= p.cu[0] && t < p.cu[p.seqs];  // rows behind the last sequence stay as they are
+  float m = -INFINITY;
+  for (int s = mg; s < p.splits; s += MG) m = fmaxf(m, p.part_lse[s * total + row]);
+#pragma unroll
+  for (int o = 16; o < 16 * MG; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.f;
+  const float m_use = m == -INFINITY ? 0.f : m;
+  for (int s = mg; s < p.splits; s += MG) {
+    const float ls = p.part_lse[s * total + row];
+    if (ls == -INFINITY) continue;  // a range that the row does not see: its partial row was never written
+    const float w = __builtin_amdgcn_exp2f(ls - m_use);
+    l += w;
+    acc += w * *reinterpret_cast<const f32x4*>(p.part_o + (s * total + row) * HD + d);
+  }
+#pragma unroll
+  for (int o = 16; o < 16 * MG; o <<= 1) {
+    l += __shfl_xor(l, o, 64);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor(acc[j], o, 64);
+  }
+  if (!live || mg != 0) return;
+  const bool none = m == -INFINITY && l == 0.f;
+  const f32x4 v = none ? f32x4{0.f, 0.f, 0.f, 0.f} : acc * (1.f / l);
+  *reinterpret_cast<uint2*>(p.o + (int64_t)t * p.orr + h * p.oh + d) =
+      uint2{pack16<F16>(v[0], v[1]), pack16<F16>(v[2], v[3])};
+  if (p.lse && d == 0) p.lse[(int64_t)h * p.new_rows + t] = none ? -INFINITY : (m_use + __log2f(l)) * LN2;
+}
+
+// ------------------------------------------------------------------------------------------------ plan
+struct Plan {
+  int rb;       // row blocks of the step kernel (0: the chunk kernel)
+  int tiles, per_tile;
+  int splits, chunk;
+  int64_t ws;   // bytes of the partials
+};
+
+int cu_count() {
+  static int cache[16] = {0};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 16) dev = 0;
+  if (cache[dev]) return cache[dev];
+  int cus = 0;
+  if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) cus = 256;
+  return cache[dev] = cus;
+}
+
+// Key ranges: n of them cost ceil(workgroups * n / slots) rounds of (tiles / n + fixed) tile times each; the n with the
+// least cost, where a round's fixed part (prologue, partial rows, their merge) is worth `fixed` tiles.
+int best_splits(int64_t wgs, int tiles, int slots, double fixed, int most) {
+  int best = 1;
+  double cost = 0;
+  for (int n = 1; n <= most && n <= tiles; ++n) {
+    const int64_t rounds = (wgs * n + slots - 1) / slots;
+    const double c = (double)rounds * ((tiles + n - 1) / n + fixed + (n > 1 ? 1.0 : 0.0));
+    if (n == 1 || c < cost * 0.98) {
+      best = n;
+      cost = c;
+    }
+  }
+  return best;
+}
+
+Plan make_plan(const mapa_attn_paged_desc& d) {
+  Plan pl = {};
+  const int group = d.heads / d.cache.heads;
+  const int cap = kv_cap(d.cache, d.batch);
+  const int64_t rows = (int64_t)d.batch.max_new * group;
+  const int slots = 2 * cu_count();
+  int unit, tiles_k;
+  int64_t wgs;
+  if (rows <= 32) {
+    pl.rb = rows <= 16 ? 1 : 2;
+    wgs = (int64_t)d.batch.seqs * d.cache.heads;
+    unit = 4 * ST;
+    tiles_k = (cap + unit - 1) / unit;
+    pl.splits = best_splits(wgs, tiles_k, slots, 4.0, 128);
+  } else {
+    pl.per_tile = std::max(1, QB / group);
+    const int64_t a = (int64_t)d.batch.new_rows / pl.per_tile + d.batch.seqs;
+    const int64_t b = (int64_t)d.batch.seqs * ((d.batch.max_new + pl.per_tile - 1) / pl.per_tile);
+    pl.tiles = (int)std::min(a, b);
+    wgs = (int64_t)pl.tiles * d.cache.heads;
+    unit = KT;
+    tiles_k = (cap + unit - 1) / unit;
+    pl.splits = best_splits(wgs, tiles_k, slots, 3.0, 64);
+  }
+  tiles_k = std::max(tiles_k, 1);
+  const int per = (tiles_k + pl.splits - 1) / pl.splits;
+  pl.splits = (tiles_k + per - 1) / per;
+  pl.chunk = per * unit;
+  pl.ws = pl.splits > 1 ? (int64_t)pl.splits * d.batch.new_rows * d.heads * (HD + 1) * 4 : 0;
+  return pl;
+}
+
+int check_desc(const mapa_attn_paged_desc* d) {
+  const char* who = "mapa_attention_paged";
+  MAPA_CHECK_ARG(d != nullptr, "%s: null descriptor", who);
+  if (int rc = check_cache(d->cache, who)) return rc;
+  if (int rc = check_batch(d->batch, who)) return rc;
+  MAPA_CHECK_ARG(d->dtype == MAPA_BF16 || d->dtype == MAPA_F16, "%s: queries must be bf16 or f16", who);
+  MAPA_CHECK_ARG(d->cache.dtype == MAPA_FP8 || d->cache.dtype == MAPA_I8 || d->cache.dtype == d->dtype,
+                 "%s: 16-bit pages must have the queries' type", who);
+  MAPA_CHECK_ARG(d->heads > 0 && d->heads <= 65535 && d->heads % d->cache.heads == 0 &&
+                     d->heads / d->cache.heads <= QB,
+                 "%s: %d query heads over %d K/V heads", who, d->heads, d->cache.heads);
+  MAPA_CHECK_ARG(d->mask_block >= 0, "%s: bad mask_block %d", who, d->mask_block);
+  MAPA_CHECK_ARG(d->scale >= 0.f && d->scale < 1e30f, "%s: bad scale %g", who, (double)d->scale);
+  return 0;
+}
+
+template <bool F16, int CK>
+void launch(const PagedArgs& a, const Plan& pl, hipStream_t stream) {
+  if (pl.rb == 0) {
+    const dim3 grid((unsigned)((int64_t)a.tiles * a.splits * a.kv_heads));
+    hipLaunchKernelGGL((attn_paged_chunk<F16, CK>), grid, dim3(NT), 0, stream, a);
+  } else {
+    const dim3 grid((unsigned)((int64_t)a.seqs * a.splits * a.kv_heads));
+    if (pl.rb == 1) hipLaunchKernelGGL((attn_paged_step<F16, CK, 1>), grid, dim3(NT), 0, stream, a);
+    else hipLaunchKernelGGL((attn_paged_step<F16, CK, 2>), grid, dim3(NT), 0, stream, a);
+  }
+}
+
+}  // namespace
+
+extern "C" int64_t mapa_attention_paged_workspace_bytes(const mapa_attn_paged_desc* d) {
+  if (check_desc(d) || d->batch.seqs == 0 || d->batch.new_rows == 0) return 0;
+  return make_plan(*d).ws;
+}
+
+extern "C" int mapa_attention_paged(const mapa_attn_paged_desc* d, hipStream_t stream) {
+  if (int rc = check_desc(d)) return rc;
+  const mapa_kv_batch& b = d->batch;
+  if (b.seqs == 0 || b.new_rows == 0 || b.max_new == 0) return 0;
+  MAPA_CHECK_ARG(d->q && d->o && (uintptr_t)d->q % 16 == 0 && (uintptr_t)d->o % 16 == 0 && d->q_rstride % 8 == 0 &&
+                     d->q_hstride % 8 == 0 && d->o_rstride % 8 == 0 && d->o_hstride % 8 == 0,
+                 "mapa_attention_paged: query / output bases and strides must keep 16-byte alignment");
+  Plan pl = make_plan(*d);
+  if (pl.splits > 1 && !(d->workspace && (uintptr_t)d->workspace % 16 == 0 && d->workspace_bytes >= pl.ws)) {
+    const int unit = pl.rb ? 4 * ST : KT;
+    pl.chunk = std::max(1, (kv_cap(d->cache, b) + unit - 1) / unit) * unit;
+    pl.splits = 1;
+  }
+  PagedArgs a = {};
+  a.page[0] = (const char*)d->cache.k; a.page[1] = (const char*)d->cache.v;
+  a.exp[0] = d->cache.k_exp; a.exp[1] = d->cache.v_exp;
+  a.table = b.table; a.kv_lens = b.kv_lens; a.cu = b.cu_new;
+  a.q = (const uint16_t*)d->q; a.o = (uint16_t*)d->o; a.lse = d->lse;
+  a.qr = d->q_rstride; a.qh = d->q_hstride; a.orr = d->o_rstride; a.oh = d->o_hstride;
+  a.fault = mapa_gemm_impl::fault_word();
+  a.c = (d->scale > 0.f ? d->scale : 0.125f) * LOG2E;
+  a.seqs = b.seqs; a.table_stride = b.table_stride; a.new_rows = b.new_rows; a.max_new = b.max_new;
+  a.cap = kv_cap(d->cache, b);
+  a.num_pages = d->cache.num_pages; a.psl = log2_of(d->cache.page_size);
+  a.heads = d->heads; a.kv_heads = d->cache.heads; a.group = d->heads / d->cache.heads;
+  a.block = d->mask_block;
+  a.splits = pl.splits; a.chunk = pl.chunk; a.tiles = pl.tiles; a.per_tile = pl.per_tile;
+  const int64_t wgs = (pl.rb ? (int64_t)b.seqs : (int64_t)pl.tiles) * a.splits * a.kv_heads;
+  MAPA_CHECK_ARG(wgs <= 0x7fffffff, "mapa_attention_paged: too many workgroups");
+  if (a.splits > 1) {
+    a.part_o = (float*)d->workspace;
+    a.part_lse = a.part_o + (int64_t)a.splits * b.new_rows * a.heads * HD;
+  }
+  const int ck = d->cache.dtype == MAPA_FP8 ? 1 : d->cache.dtype == MAPA_I8 ? 2 : 0;
+  const bool f16 = d->dtype == MAPA_F16;
+  if (f16) {
+    if (ck == 0) launch<true, 0>(a, pl, stream);
+    else if (ck == 1) launch<true, 1>(a, pl, stream);
+    else launch<true, 2>(a, pl, stream);
+  } else {
+    if (ck == 0) launch<false, 0>(a, pl, stream);
+    else if (ck == 1) launch<false, 1>(a, pl, stream);
+    else launch<false, 2>(a, pl, stream);
+  }
+  MAPA_CHECK_LAUNCH("mapa_attention_paged");
+  if (a.splits > 1) {
+    const int64_t rows = (int64_t)b.new_rows * a.heads;
+    const int mg = a.splits >= 8 ? 4 : 1;
+    const int64_t per = NT / (16 * mg);
+    const dim3 grid((unsigned)((rows + per - 1) / per));
+    if (f16 && mg == 4) hipLaunchKernelGGL((attn_paged_merge<true, 4>), grid, dim3(NT), 0, stream, a);
+    else if (f16) hipLaunchKernelGGL((attn_paged_merge<true, 1>), grid, dim3(NT), 0, stream, a);
+    else if (mg == 4) hipLaunchKernelGGL((attn_paged_merge<false, 4>), grid, dim3(NT), 0, stream, a);
+    else hipLaunchKernelGGL((attn_paged_merge<false, 1>), grid, dim3(NT), 0, stream, a);
+    MAPA_CHECK_LAUNCH("mapa_attention_paged (merge)");
+  }
+  return 0;
+}

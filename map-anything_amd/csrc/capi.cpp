@@ -56,6 +56,9 @@ extern "C" int mapa_stream_check(hipStream_t stream, const char* what) {
   if (f & MAPA_FAULT_LN_BARRIER)
     return mapa_set_error("%s: a LayerNorm-fused GEMM band barrier timed out (its LayerNorm rows are invalid)",
                           what ? what : "launch");
+  if (f & MAPA_FAULT_KV_RANGE)
+    return mapa_set_error("%s: a paged K/V cache call met a page, length or row offset outside what the host stated",
+                          what ? what : "launch");
   if (f) return mapa_set_error("%s: device fault word 0x%x", what ? what : "launch", (unsigned)f);
   return 0;
 }

@@ -6,6 +6,7 @@ raw device pointers on torch's current HIP stream (torch is the allocator and st
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from typing import Optional
@@ -15,7 +16,7 @@ import torch
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libmapa.so")
 _lib = None
 
-F32, BF16, BF16X3, F16, F16X2 = 0, 1, 2, 3, 4
+F32, BF16, BF16X3, F16, F16X2, FP8, I8 = 0, 1, 2, 3, 4, 5, 6
 A_DENSE, A_CONV3X3 = 0, 1
 OUT_ROWMAJOR, OUT_PIXSHUF = 0, 1
 ACT_NONE, ACT_GELU, ACT_RELU, ACT_GELU_POST = 0, 1, 2, 3
@@ -35,9 +36,15 @@ EXPORTED = (
     "mapa_comm_unique_id_bytes", "mapa_comm_get_unique_id", "mapa_comm_init", "mapa_comm_allgather_kv",
     "mapa_comm_broadcast", "mapa_comm_check", "mapa_comm_destroy",
     "mapa_resize_plan_bytes", "mapa_resize_plan_build", "mapa_resize_workspace_bytes", "mapa_resize_normalize",
+    "mapa_rope_axes", "mapa_kv_cache_write", "mapa_kv_cache_read", "mapa_attention_paged",
+    "mapa_attention_paged_workspace_bytes",
 )
 FAULT_LN_BARRIER = 1  # include/mapa.h MAPA_FAULT_LN_BARRIER
 FAULT_F16_RANGE = 2  # include/mapa.h MAPA_FAULT_F16_RANGE
+FAULT_KV_RANGE = 4  # include/mapa.h MAPA_FAULT_KV_RANGE
+ROPE_AXIAL, ROPE_HALF, ROPE_INTERLEAVED = 0, 1, 2  # include/mapa.h MAPA_ROPE_*
+POS_I64, POS_F32 = 0, 1  # include/mapa.h MAPA_POS_*
+ROPE_MAX_AXES, ROPE_MAX_PAIRS = 4, 128
 RESAMPLE_LANCZOS, RESAMPLE_BILINEAR, RESAMPLE_BICUBIC = 1, 2, 3  # include/mapa.h MAPA_RESAMPLE_* (PIL numbering)
 
 
@@ -75,6 +82,48 @@ class AttnDesc(ctypes.Structure):
         ("lse", ctypes.c_void_p), ("kv_nseg", ctypes.c_int), ("kv_seg_start", ctypes.c_int * 16),
         ("kv_seg_len", ctypes.c_int * 16), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64),
         ("scale", ctypes.c_float),
+    ]
+
+
+class RopeAxesDesc(ctypes.Structure):
+    """include/mapa.h mapa_rope_axes_desc"""
+    _fields_ = [
+        ("dtype", ctypes.c_int), ("batch", ctypes.c_int), ("tokens", ctypes.c_int), ("head_dim", ctypes.c_int),
+        ("x", ctypes.c_void_p * 2), ("y", ctypes.c_void_p * 2), ("heads", ctypes.c_int * 2),
+        ("x_bstride", ctypes.c_int64 * 2), ("x_hstride", ctypes.c_int64 * 2), ("x_nstride", ctypes.c_int64 * 2),
+        ("y_bstride", ctypes.c_int64 * 2), ("y_hstride", ctypes.c_int64 * 2), ("y_nstride", ctypes.c_int64 * 2),
+        ("positions", ctypes.c_void_p), ("pos_dtype", ctypes.c_int), ("pos_bstride", ctypes.c_int64),
+        ("pos_nstride", ctypes.c_int64), ("pos_astride", ctypes.c_int64), ("axes", ctypes.c_int),
+        ("section", ctypes.c_int * ROPE_MAX_AXES), ("layout", ctypes.c_int), ("inverse", ctypes.c_int),
+        ("freq", ctypes.c_double * ROPE_MAX_PAIRS),
+    ]
+
+
+class KVCacheDesc(ctypes.Structure):
+    """include/mapa.h mapa_kv_cache"""
+    _fields_ = [
+        ("dtype", ctypes.c_int), ("heads", ctypes.c_int), ("page_size", ctypes.c_int), ("num_pages", ctypes.c_int),
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_exp", ctypes.c_void_p), ("v_exp", ctypes.c_void_p),
+    ]
+
+
+class KVBatchDesc(ctypes.Structure):
+    """include/mapa.h mapa_kv_batch"""
+    _fields_ = [
+        ("seqs", ctypes.c_int), ("table_stride", ctypes.c_int), ("table", ctypes.c_void_p),
+        ("kv_lens", ctypes.c_void_p), ("cu_new", ctypes.c_void_p), ("new_rows", ctypes.c_int),
+        ("max_new", ctypes.c_int), ("max_kv", ctypes.c_int),
+    ]
+
+
+class AttnPagedDesc(ctypes.Structure):
+    """include/mapa.h mapa_attn_paged_desc"""
+    _fields_ = [
+        ("cache", KVCacheDesc), ("batch", KVBatchDesc), ("dtype", ctypes.c_int), ("heads", ctypes.c_int),
+        ("q", ctypes.c_void_p), ("o", ctypes.c_void_p), ("q_rstride", ctypes.c_int64), ("q_hstride", ctypes.c_int64),
+        ("o_rstride", ctypes.c_int64), ("o_hstride", ctypes.c_int64), ("lse", ctypes.c_void_p),
+        ("scale", ctypes.c_float), ("mask_block", ctypes.c_int), ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
     ]
 
 
@@ -171,6 +220,13 @@ def load_library(path: Optional[str] = None):
     L.mapa_resize_workspace_bytes.argtypes = [vp]
     L.mapa_resize_workspace_bytes.restype = i64
     L.mapa_resize_normalize.argtypes = [vp, i64, vp, vp, vp, vp, vp, vp, vp, i64, vp]
+    L.mapa_rope_axes.argtypes = [ctypes.POINTER(RopeAxesDesc), vp]
+    pc, pb = ctypes.POINTER(KVCacheDesc), ctypes.POINTER(KVBatchDesc)
+    L.mapa_kv_cache_write.argtypes = [pc, pb, vp, vp, i, i64, i64, i64, i64, vp]
+    L.mapa_kv_cache_read.argtypes = [pc, pb, vp, i, vp, vp, i, i64, i64, i64, i64, vp]
+    L.mapa_attention_paged.argtypes = [ctypes.POINTER(AttnPagedDesc), vp]
+    L.mapa_attention_paged_workspace_bytes.argtypes = [ctypes.POINTER(AttnPagedDesc)]
+    L.mapa_attention_paged_workspace_bytes.restype = i64
     _lib = L
     return L
 
@@ -222,6 +278,16 @@ def stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Context in which `device` is the current one (its current stream is the one launched on)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(device)
+
+
 def dt_code(dtype: torch.dtype) -> int:
     if dtype == torch.bfloat16:
         return BF16
@@ -241,6 +307,9 @@ def _fault_message(bits: int) -> str:
         return ("a binary16 operand (the TF32-equivalent heads, or the fp16 recipe) left binary16's range (include/"
                 "mapa.h MAPA_FAULT_F16_RANGE): this call's outputs were discarded; head_precision='fp32' runs the heads "
                 "fp32-exact")
+    if bits & FAULT_KV_RANGE:
+        return ("a paged K/V cache call met a page number, length or row offset outside what the host stated "
+                "(include/mapa.h MAPA_FAULT_KV_RANGE): the rows concerned were skipped or are not valid")
     return f"device fault word 0x{bits:x}"
 
 
@@ -863,3 +932,46 @@ def rope2d(tokens, positions, B, H, N, D, sb, sh, sn, base, f0):
         raise NativeError("rope2d: positions must be contiguous int64 (B, N, 2)")
     check(lib().mapa_rope2d(ptr(tokens), dt_code(tokens.dtype), B, H, N, D, sb, sh, sn, ptr(positions), float(base),
                             float(f0), stream()), "mapa_rope2d")
+
+
+def rope_axes(d: RopeAxesDesc):
+    """Rotary positions with several axes (include/mapa.h mapa_rope_axes_desc); uniception's RoPEAxes fills it."""
+    tok = _tic()
+    check(lib().mapa_rope_axes(ctypes.byref(d), stream()), "mapa_rope_axes")
+    _toc(tok, "rope_axes")
+
+
+def kv_cache_write(cache: KVCacheDesc, batch: KVBatchDesc, k, v):
+    """New rows k, v (rows, heads, 64) into the pages of a paged K/V cache (mapanything.kv_cache.PagedKVCache)."""
+    tok = _tic()
+    check(lib().mapa_kv_cache_write(ctypes.byref(cache), ctypes.byref(batch), k.data_ptr(), v.data_ptr(),
+                                    dt_code(k.dtype), k.stride(0), k.stride(1), v.stride(0), v.stride(1), stream()),
+          "mapa_kv_cache_write")
+    _toc(tok, "kv_cache_write")
+
+
+def kv_cache_read(cache: KVCacheDesc, batch: KVBatchDesc, cu_rows, rows: int, k, v):
+    """Cached rows back into k, v (rows, heads, 64) (mapanything.kv_cache.PagedKVCache)."""
+    tok = _tic()
+    check(lib().mapa_kv_cache_read(ctypes.byref(cache), ctypes.byref(batch), cu_rows.data_ptr(), rows, k.data_ptr(),
+                                   v.data_ptr(), dt_code(k.dtype), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                                   stream()), "mapa_kv_cache_read")
+    _toc(tok, "kv_cache_read")
+
+
+def attention_paged(cache: KVCacheDesc, batch: KVBatchDesc, q, o, *, lse=None, scale=None, mask_block=0):
+    """Attention of the batch's new tokens q (rows, heads, 64) over their sequences' pages.  The partials' workspace is
+    a tensor of this call alone: the allocator orders its reuse on the current stream, and inside a graph capture it
+    belongs to that graph's pool, so two graphs never share one."""
+    d = AttnPagedDesc(cache=cache, batch=batch, dtype=dt_code(q.dtype), heads=q.shape[1], q=q.data_ptr(), o=o.data_ptr(),
+                      q_rstride=q.stride(0), q_hstride=q.stride(1), o_rstride=o.stride(0), o_hstride=o.stride(1),
+                      lse=None if lse is None else lse.data_ptr(), scale=0.0 if scale is None else scale,
+                      mask_block=mask_block)
+    L = lib()
+    need = L.mapa_attention_paged_workspace_bytes(ctypes.byref(d))
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        d.workspace, d.workspace_bytes = ws.data_ptr(), need
+    tok = _tic()
+    check(L.mapa_attention_paged(ctypes.byref(d), stream()), "mapa_attention_paged")
+    _toc(tok, "attention_paged")

@@ -39,3 +39,144 @@ class RoPE2D:
 
 
 cuRoPE2D = RoPE2D  # curope2d.py:31: the CUDA class the reference prefers when its extension is built
+
+
+class _RoPEAxesTurn(torch.autograd.Function):
+    """One turn of one or two tensors, out of place; its backward is the same turn the other way."""
+
+    @staticmethod
+    def forward(ctx, rope, inverse, positions, tokens, keys):
+        ctx.rope, ctx.inverse = rope, inverse
+        ctx.save_for_backward(positions)
+        ctx.set_materialize_grads(False)
+        return rope._turn(tokens, keys, positions, inverse)
+
+    @staticmethod
+    def backward(ctx, g_tokens, g_keys=None):
+        (positions,) = ctx.saved_tensors
+        first, second = (g_tokens, g_keys) if g_tokens is not None else (g_keys, None)
+        if first is None:
+            return (None,) * 5
+        a, b = _RoPEAxesTurn.apply(ctx.rope, not ctx.inverse, positions, first, second)
+        return (None, None, None) + ((a, b) if g_tokens is not None else (None, a))
+
+
+class RoPEAxes:
+    """Rotary positions with several axes (time, row, column, ...): RoPE2D's rotation for any split of the head's pairs
+    over up to four axes, differentiable, on the gfx950 kernel `mapa_rope_axes` (include/mapa.h).  RoPE2D is
+    `RoPEAxes((D // 4, D // 4), freq)`.
+
+        rope = RoPEAxes(sections=(8, 12, 12), freq=10000.0)     # 32 pairs: time, row, column
+        q, k = rope(q, positions, k)                            # (B, heads, N, 64) each, positions (B, N, 3)
+
+    sections: pairs per axis; dims behind the last pair pass through.  layout: the columns of a pair (u, v) —
+    "axial" (each axis' own block [u | v], RoPE2D's), "half" (u in the first half of the rotated dims, v in the second)
+    or "interleaved" (neighbours).  spectrum: pair j of an axis of n pairs turns by F0 / freq^(j / n) per unit of
+    position ("axis", RoPE2D's), or one table runs through the pairs of all axes ("shared").
+
+    tokens / keys: (B, H, N, D) fp32, bf16 or fp16 with a contiguous head dim and any other strides (a view of packed
+    qkv rows), the head counts of the two may differ.  positions: (B, N, axes) or (N, axes), integer or fp32; angles are
+    formed in 64 bits.  Returns new tensors, or with inplace=True (not for tensors that need a gradient) the rotated
+    inputs, as RoPE2D does."""
+
+    _LAYOUTS = {"axial": nat.ROPE_AXIAL, "half": nat.ROPE_HALF, "interleaved": nat.ROPE_INTERLEAVED}
+
+    def __init__(self, sections, freq: float = 100.0, F0: float = 1.0, layout: str = "axial", spectrum: str = "axis"):
+        sections = tuple(int(n) for n in sections)
+        if not 1 <= len(sections) <= nat.ROPE_MAX_AXES or min(sections) < 1 or sum(sections) > nat.ROPE_MAX_PAIRS:
+            raise ValueError(f"RoPEAxes: sections {sections} must be 1 to {nat.ROPE_MAX_AXES} positive pair counts, "
+                             f"{nat.ROPE_MAX_PAIRS} pairs at most")
+        if layout not in self._LAYOUTS:
+            raise ValueError(f"RoPEAxes: layout must be one of {sorted(self._LAYOUTS)}, got {layout!r}")
+        if spectrum not in ("axis", "shared"):
+            raise ValueError(f"RoPEAxes: spectrum must be 'axis' or 'shared', got {spectrum!r}")
+        if not float(freq) > 0:
+            raise ValueError(f"RoPEAxes: freq must be positive, got {freq}")
+        self.sections, self.base, self.F0 = sections, float(freq), float(F0)
+        self.layout, self.spectrum = layout, spectrum
+        pairs = sum(sections)
+        if spectrum == "axis":
+            part = [j / n for n in sections for j in range(n)]
+        else:
+            part = [i / pairs for i in range(pairs)]
+        d = nat.RopeAxesDesc(axes=len(sections), layout=self._LAYOUTS[layout])
+        for i, n in enumerate(sections):
+            d.section[i] = n
+        for i, x in enumerate(part):
+            d.freq[i] = self.F0 * self.base ** -x
+        self._desc = d
+
+    def __call__(self, tokens, positions, keys=None, inplace: bool = False):
+        return self.forward(tokens, positions, keys, inplace)
+
+    def forward(self, tokens, positions, keys=None, inplace: bool = False):
+        for name, t in (("tokens", tokens), ("keys", keys)):
+            if t is None:
+                continue
+            if t.ndim != 4 or 2 * sum(self.sections) > t.shape[3]:
+                raise ValueError(f"RoPEAxes: {name} {tuple(t.shape)} must be (B, H, N, D) with D >= "
+                                 f"{2 * sum(self.sections)}")
+            if t.device != tokens.device or t.dtype != tokens.dtype or t.shape[2:] != tokens.shape[2:] or \
+                    t.shape[0] != tokens.shape[0]:
+                raise ValueError("RoPEAxes: tokens and keys must share device, dtype, batch, length and head dim")
+            if t.stride(3) != 1 and t.shape[3] > 1:
+                raise ValueError("RoPEAxes: the head dimension must be contiguous")
+        B, _, N, _ = tokens.shape
+        if positions.ndim == 2:
+            positions = positions[None]
+        if positions.ndim != 3 or positions.shape[0] not in (1, B) or positions.shape[1:] != (N, len(self.sections)):
+            raise ValueError(f"RoPEAxes: positions {tuple(positions.shape)} do not match tokens (B={B}, N={N}) and "
+                             f"{len(self.sections)} axes")
+        if positions.dtype != torch.int64 and positions.dtype != torch.float32:
+            if positions.is_floating_point() or positions.is_complex() or positions.dtype == torch.bool:
+                raise ValueError(f"RoPEAxes: positions must be integer or fp32, got {positions.dtype}")
+            positions = positions.to(torch.int64)
+        if positions.device != tokens.device:
+            positions = positions.to(tokens.device)
+        needs = torch.is_grad_enabled() and (tokens.requires_grad or (keys is not None and keys.requires_grad))
+        if inplace:
+            if needs:
+                raise ValueError("RoPEAxes: inplace rotation of a tensor that needs a gradient")
+            for t in (tokens, keys):
+                if t is not None and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+                    raise ValueError("RoPEAxes: inplace rotation of an expanded tensor")
+            self._run(tokens, keys, positions, False, tokens, keys)
+            return tokens if keys is None else (tokens, keys)
+        if needs:
+            out = _RoPEAxesTurn.apply(self, False, positions.detach(), tokens, keys)
+        else:
+            out = self._turn(tokens, keys, positions, False)
+        return out[0] if keys is None else out
+
+    def _turn(self, tokens, keys, positions, inverse):
+        a = tokens if tokens.stride(3) == 1 else tokens.contiguous()  # a gradient may come expanded
+        b = keys if keys is None or keys.stride(3) == 1 else keys.contiguous()
+        ya, yb = _like(a), None if b is None else _like(b)
+        self._run(a, b, positions, inverse, ya, yb)
+        return ya, yb
+
+    def _run(self, a, b, positions, inverse, ya, yb):
+        if not a.is_cuda:
+            raise nat.NativeError("RoPEAxes: tensors must be on the GPU; there is no CPU path")
+        B, _, N, D = a.shape
+        d = nat.RopeAxesDesc.from_buffer_copy(self._desc)
+        d.dtype, d.batch, d.tokens, d.head_dim, d.inverse = nat.dt_code(a.dtype), B, N, D, int(inverse)
+        for i, (x, y) in enumerate(((a, ya), (b, yb))):
+            if x is not None:
+                d.x[i], d.y[i], d.heads[i] = x.data_ptr(), y.data_ptr(), x.shape[1]
+                d.x_bstride[i], d.x_hstride[i], d.x_nstride[i], _ = x.stride()
+                d.y_bstride[i], d.y_hstride[i], d.y_nstride[i], _ = y.stride()
+        d.positions = positions.data_ptr()
+        d.pos_dtype = nat.POS_F32 if positions.dtype == torch.float32 else nat.POS_I64
+        pb, d.pos_nstride, d.pos_astride = positions.stride()
+        d.pos_bstride = pb if positions.shape[0] > 1 else 0
+        with nat.on_device(a.device):
+            nat.rope_axes(d)
+
+
+def _like(x):
+    """An empty (B, H, N, D) tensor laid out as x is: heads inside tokens, or tokens inside heads."""
+    B, H, N, D = x.shape
+    if x.stride(1) < x.stride(2):
+        return x.new_empty(B, N, H, D).transpose(1, 2)
+    return x.new_empty(B, H, N, D)
