@@ -17,6 +17,7 @@
 //  * keys are cut into ranges of `chunk` when rows alone do not fill the chip; attn_paged_merge joins the fp32 partials
 //    in a fixed order.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "paged.h"
@@ -43,16 +44,17 @@ struct PagedArgs {
   uint16_t* o;
   float* lse;
   int64_t qr, qh, orr, oh;
-  float* part_o;    // [splits][new_rows * heads][64]
-  float* part_lse;  // [splits][new_rows * heads], log2 domain
+  float* part_o;    // [slot][rows of a workgroup][64], normalised
+  float* part_lse;  // [slot][rows of a workgroup], log2 domain
   unsigned* fault;
   float c;  // scale * log2(e)
   int seqs, table_stride, new_rows, max_new, cap, num_pages, psl;
   int heads, kv_heads, group;
   int block;    // mask_block
-  int splits, chunk;
-  int tiles;    // row tiles of the grid (upper bound)
-  int per_tile; // tokens of a row tile
+  int splits, chunk;  // key ranges of a split task, keys of a range
+  int whole;     // tasks [0, whole) of the chunk kernel walk all their keys, the others are split
+  int tiles;     // row tiles of the grid (upper bound)
+  int per_tile;  // tokens of a row tile
 };
 
 typedef short s4v __attribute__((ext_vector_type(4)));
@@ -126,6 +128,44 @@ template <bool F16>
 __device__ __forceinline__ uint32_t pack16(float a, float b) {
   return pack_lp2(F16, a, b);
 }
+// Row tile of the chunk kernel -> (sequence, its first packed row, its new tokens, tile in it), by a wave-wide prefix sum
+// over the sequences' tile counts, 64 at a time; seq -1: no such tile.
+struct RowTile {
+  int seq, c0, nq, tile;
+};
+__device__ __forceinline__ RowTile find_tile(const PagedArgs& p, int tile, int lane) {
+  int before = 0;
+#pragma unroll 1
+  for (int s0 = 0; s0 < p.seqs; s0 += 64) {
+    const int s = s0 + lane;
+    int q0 = 0, n = 0;
+    if (s < p.seqs) {
+      q0 = p.cu[s];
+      n = new_tokens(p, q0, p.cu[s + 1]);
+    }
+    int sum = (n + p.per_tile - 1) / p.per_tile;
+    const int own = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += up;
+    }
+    const uint64_t past = __ballot(before + sum > tile);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      return RowTile{s0 + l, __builtin_amdgcn_readlane(q0, l), __builtin_amdgcn_readlane(n, l),
+                     tile - before - __builtin_amdgcn_readlane(sum - own, l)};
+    }
+    before += __builtin_amdgcn_readlane(sum, 63);
+  }
+  return RowTile{-1, 0, 0, 0};
+}
+// task of the chunk kernel -> (K/V head, row tile): row tiles inside heads (they share K/V), the last ones (the longest
+// key ranges under a causal mask) first
+__device__ __forceinline__ void task_coords(const PagedArgs& p, int task, int& hk, int& tile) {
+  hk = task / p.tiles;
+  tile = p.tiles - 1 - (task - hk * p.tiles);
+}
 
 // ------------------------------------------------------------------------------------------------ chunk
 // CK: 0 = 16-bit pages of the query's type, 1 = e4m3, 2 = int8
@@ -136,45 +176,24 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hl = lane >> 5, l32 = lane & 31;
 
-  // work: (K/V head, key range, row tile), row tiles innermost (they share K/V), the last ones (the longest key
-  // ranges under a causal mask) first
-  const int nblk = p.tiles * p.splits * p.kv_heads;
-  const int w = mapa_idx::xcd_remap(blockIdx.x, nblk);
-  int tile = w % p.tiles;
-  const int hs = w / p.tiles, split = hs % p.splits, hk = hs / p.splits;
-  tile = p.tiles - 1 - tile;
-
-  // row tile -> (sequence, tile in it): a wave-wide prefix sum over the sequences' tile counts, 64 at a time
-  int b = -1, nq = 0, c0 = 0;
-  {
-    int before = 0;
-#pragma unroll 1
-    for (int s0 = 0; s0 < p.seqs; s0 += 64) {
-      const int s = s0 + lane;
-      int q0 = 0, n = 0;
-      if (s < p.seqs) {
-        q0 = p.cu[s];
-        n = new_tokens(p, q0, p.cu[s + 1]);
-      }
-      int sum = (n + p.per_tile - 1) / p.per_tile;
-      const int own = sum;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int up = __shfl_up(sum, o, 64);
-        if (lane >= o) sum += up;
-      }
-      const uint64_t past = __ballot(before + sum > tile);
-      if (past) {
-        const int l = __builtin_ctzll(past);
-        b = s0 + l;
-        nq = __builtin_amdgcn_readlane(n, l);
-        c0 = __builtin_amdgcn_readlane(q0, l);
-        tile -= before + __builtin_amdgcn_readlane(sum - own, l);
-        break;
-      }
-      before += __builtin_amdgcn_readlane(sum, 63);
-    }
+  // whole tasks first, each XCD a contiguous run of them; then the split ones, range-major, so that workgroups which
+  // share a K/V range run together on one XCD
+  int task, split = 0, slot = -1;
+  if ((int)blockIdx.x < p.whole) {
+    task = mapa_idx::xcd_remap(blockIdx.x, p.whole);
+  } else {
+    const int rest = p.tiles * p.kv_heads - p.whole;
+    const int v = mapa_idx::xcd_remap(blockIdx.x - p.whole, rest * p.splits);
+    split = v / rest;
+    const int j = v - split * rest;
+    task = p.whole + j;
+    slot = j * p.splits + split;
   }
+  int hk, tile;
+  task_coords(p, task, hk, tile);
+  const RowTile rt0 = find_tile(p, tile, lane);
+  const int b = rt0.seq, nq = rt0.nq, c0 = rt0.c0;
+  tile = rt0.tile;
   if (b < 0) return;
   const int len = __builtin_amdgcn_readfirstlane(checked_len(p.kv_lens[b], p.cap, p.fault));
   const int t0 = tile * p.per_tile;                       // first token of the tile, in its sequence
@@ -182,7 +201,7 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
   const int pos0 = len - nq + t0;                         // position of the first token
   const int lim_lo = key_limit(pos0, len, p.block);
   const int lim_hi = key_limit(pos0 + (rows - 1) / p.group, len, p.block);
-  const int k_begin = split * p.chunk, k_end = min(k_begin + p.chunk, lim_hi);
+  const int k_begin = split * p.chunk, k_end = slot < 0 ? lim_hi : min(k_begin + p.chunk, lim_hi);
 
   // this lane's row
   const int r = wave * 32 + l32;
@@ -190,11 +209,8 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
   const int rt = rc / p.group, rg = rc - rt * p.group;
   const int tok = c0 + t0 + rt, head = hk * p.group + rg;
   const int limit = key_limit(pos0 + rt, len, p.block);
-  const int64_t prow = ((int64_t)split * p.new_rows + tok) * p.heads + head;  // row of the partials
-  if (k_begin >= k_end) {  // no key of this range is seen by any row of the tile
-    if (p.splits > 1) {
-      if (r < rows && hl == 0) p.part_lse[prow] = -INFINITY;
-    } else if (r < rows) {
+  if (k_begin >= k_end) {  // no key of this range is seen by any row of the tile (the merge knows which ranges are)
+    if (slot < 0 && r < rows) {
       uint16_t* o = p.o + (int64_t)tok * p.orr + head * p.oh + hl * 32;
 #pragma unroll
       for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(o)[i] = uint4{0, 0, 0, 0};
@@ -228,22 +244,32 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
 
   const char* zero = reinterpret_cast<const char*>(g_mapa_zero_page);
   // 16-bit pages: 16 pieces of 8 rows x 128 B (K: 0..7, V: 8..15), four per wave; the 16-B column is XOR-swizzled on
-  // the source so that the LDS image stays lane-linear
-  auto stage16 = [&](int slot, int kt) __attribute__((always_inline)) {
-    char* dst = lds + slot * 2 * TILE;
+  // the source so that the LDS image stays lane-linear.  A piece lies in one page: a scalar base and a fixed offset per
+  // lane, but for the tile that the sequence ends in, whose rows past the end come from the zero page.
+  const int prow8 = lane >> 3;
+  const int koff = prow8 * 128 + (((lane & 7) ^ (((wave & 1) * 4 + (lane >> 4)) & 7)) << 4);
+  const int voff = prow8 * 128 + (((lane & 7) ^ (((lane >> 4) & 1) << 2)) << 4);
+  auto stage16 = [&](int slot_, int kt) __attribute__((always_inline)) {
+    char* dst = lds + slot_ * 2 * TILE;
     const int key0 = kt * KT;
     need_window(key0);
+    const bool full = key0 + KT <= len;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int k8 = (i * 4 + wave) * 8;  // first tile row of the piece (K and V alike)
-      const int row = k8 + (lane >> 3), pos = lane & 7;
-      const int kc = (pos ^ ((row >> 1) & 7)) * 16, vc = (pos ^ (((row >> 1) & 1) << 2)) * 16;
       const int64_t at = cache_row(key0 + k8) * 128;
-      const bool in = key0 + row < len;
-      const char* ks = in ? p.page[0] + at + (lane >> 3) * 128 + kc : zero;
-      const char* vs = in ? p.page[1] + at + (lane >> 3) * 128 + vc : zero;
-      __builtin_amdgcn_global_load_lds(ks, (lds_ptr_t)(dst + k8 * 128), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(vs, (lds_ptr_t)(dst + TILE + k8 * 128), 16, 0, 0);
+      const char* kp = p.page[0] + at;
+      const char* vp = p.page[1] + at;
+      if (full) {
+        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)kp, 0, 1024, 0x00020000);
+        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)vp, 0, 1024, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_ptr_t)(dst + k8 * 128), 16, koff, 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_ptr_t)(dst + TILE + k8 * 128), 16, voff, 0, 0, 0);
+      } else {
+        const bool in = key0 + k8 + prow8 < len;
+        __builtin_amdgcn_global_load_lds(in ? kp + koff : zero, (lds_ptr_t)(dst + k8 * 128), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds(in ? vp + voff : zero, (lds_ptr_t)(dst + TILE + k8 * 128), 16, 0, 0);
+      }
     }
   };
   // 8-bit pages: thread -> tile row tid / 4, 16 codes; loaded one tile ahead, decoded after the tile's products
@@ -253,13 +279,12 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
   auto load8 = [&](int kt) __attribute__((always_inline)) {
     const int key0 = kt * KT;
     need_window(key0);
-    const int row = tid >> 2;
-    const int64_t at = cache_row(key0 + wave * 16) + (lane >> 2);
-    cin = key0 + row < len;
+    const int64_t at = cache_row(key0 + wave * 16);  // scalar; 16 rows of 64 B are contiguous
+    cin = key0 + (tid >> 2) < len;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      creg[x] = *reinterpret_cast<const uint4*>(p.page[x] + at * 64 + (lane & 3) * 16);
-      ereg[x] = p.exp[x][at];
+      creg[x] = reinterpret_cast<const uint4*>(p.page[x] + at * 64)[lane];
+      ereg[x] = (p.exp[x] + at)[lane >> 2];
     }
   };
   auto store8 = [&](int slot) __attribute__((always_inline)) {
@@ -354,7 +379,7 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
     bf16x8 pf[2][2];
     float ls;
     auto exp_pack = [&]() __attribute__((always_inline)) {
-      float a[4];
+      float a[4];  // four sums, seeded with the first values
       const float nm = -m_ref;
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
@@ -479,7 +504,7 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
   }
-  if (p.splits == 1) {
+  if (slot < 0) {
     uint16_t* obase = p.o + (int64_t)tok * p.orr + head * p.oh;
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt)
@@ -498,6 +523,7 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
       }
     if (p.lse && r < rows && hl == 0) p.lse[(int64_t)head * p.new_rows + tok] = lse2 * LN2;
   } else if (r < rows) {
+    const int64_t prow = (int64_t)slot * QB + r;
     float* po = p.part_o + prow * HD;
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt)
@@ -542,15 +568,11 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
     head[rb] = hk * p.group + r - rt * p.group;
     limit[rb] = key_limit(pos0 + rt, len, p.block);
   }
-  if (k_begin >= k_end) {  // uniform: the whole workgroup leaves
-    for (int i = tid; i < rows * 8; i += NT) {
+  if (k_begin >= k_end) {  // uniform: the whole workgroup leaves (the merge knows which ranges are empty)
+    for (int i = tid; p.splits == 1 && i < rows * 8; i += NT) {
       const int r = i >> 3, rt = r / p.group, h = hk * p.group + r - rt * p.group, t = c0 + rt;
-      if (p.splits > 1) {
-        if ((i & 7) == 0) p.part_lse[((int64_t)split * p.new_rows + t) * p.heads + h] = -INFINITY;
-      } else {
-        reinterpret_cast<uint4*>(p.o + (int64_t)t * p.orr + h * p.oh)[i & 7] = uint4{0, 0, 0, 0};
-        if (p.lse && (i & 7) == 0) p.lse[(int64_t)h * p.new_rows + t] = -INFINITY;
-      }
+      reinterpret_cast<uint4*>(p.o + (int64_t)t * p.orr + h * p.oh)[i & 7] = uint4{0, 0, 0, 0};
+      if (p.lse && (i & 7) == 0) p.lse[(int64_t)h * p.new_rows + t] = -INFINITY;
     }
     return;
   }
@@ -784,7 +806,7 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
           uint2{pack16<F16>(v[0], v[1]), pack16<F16>(v[2], v[3])};
       if (p.lse && d == 0) p.lse[(int64_t)h * p.new_rows + t] = lse2 * LN2;
     } else {
-      const int64_t pr = ((int64_t)split * p.new_rows + t) * p.heads + h;
+      const int64_t pr = (((int64_t)b * p.kv_heads + hk) * p.splits + split) * RS + row;
       *reinterpret_cast<f32x4*>(p.part_o + pr * HD + d) = v;
       if (d == 0) p.part_lse[pr] = lse2;
     }
@@ -792,49 +814,103 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
 }
 
 // ------------------------------------------------------------------------------------------------ merge
-// 16 lanes x 4 columns per row, MG groups of them over every MG-th key range, joined by a fixed butterfly.
-template <bool F16, int MG>
-__global__ void __launch_bounds__(NT) attn_paged_merge(PagedArgs p) {
-  const int64_t total = (int64_t)p.new_rows * p.heads;
-  const int64_t e = (int64_t)blockIdx.x * (NT / (16 * MG)) + threadIdx.x / (16 * MG);
-  const int64_t row = e < total ? e : total - 1;
-  const int d = (threadIdx.x & 15) * 4, mg = (threadIdx.x >> 4) % MG;
-  const int t = (int)(row / p.heads), h = (int)(row % p.heads);
-  const bool live = e < total && t >= p.cu[0] && t < p.cu[p.seqs];  // rows behind the last sequence stay as they are
-  float m = -INFINITY;
-  for (int s = mg; s < p.splits; s += MG) m = fmaxf(m, p.part_lse[s * total + row]);
-#pragma unroll
-  for (int o = 16; o < 16 * MG; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+// One wave per row: four groups of 16 lanes x 4 columns, group g over the key ranges g, g + 4, ...; 32 ranges' partials
+// are in flight at once, joined in a fixed order.  `first`: the row in its first range's slot, `n`: ranges with a key
+// that the row sees.
+template <bool F16, int ROWS>
+__device__ __forceinline__ void merge_row(const PagedArgs& p, int64_t first, int n, int tok, int head, int lane) {
+  const int d = (lane & 15) * 4, g = lane >> 4;
+  float m = -INFINITY, l = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-  const float m_use = m == -INFINITY ? 0.f : m;
-  for (int s = mg; s < p.splits; s += MG) {
-    const float ls = p.part_lse[s * total + row];
-    if (ls == -INFINITY) continue;  // a range that the row does not see: its partial row was never written
-    const float w = __builtin_amdgcn_exp2f(ls - m_use);
-    l += w;
-    acc += w * *reinterpret_cast<const f32x4*>(p.part_o + (s * total + row) * HD + d);
+#pragma unroll 1
+  for (int s0 = 0; s0 < n; s0 += 32) {
+    float ls[8];
+    f32x4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int s = s0 + 4 * i + g;
+      ls[i] = -INFINITY;
+      v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (s < n) {
+        const int64_t at = first + (int64_t)s * ROWS;
+        ls[i] = p.part_lse[at];
+        v[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * HD + d);
+      }
+    }
+    float mx = m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mx = fmaxf(mx, ls[i]);
+    const float use = mx == -INFINITY ? 0.f : mx;
+    const float keep = __builtin_amdgcn_exp2f(m - use);
+    l *= keep;
+    acc *= keep;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float w = __builtin_amdgcn_exp2f(ls[i] - use);
+      l += w;
+      acc += w * v[i];
+    }
+    m = mx;
   }
 #pragma unroll
-  for (int o = 16; o < 16 * MG; o <<= 1) {
-    l += __shfl_xor(l, o, 64);
+  for (int o = 16; o < 64; o <<= 1) {
+    const float m2 = __shfl_xor(m, o, 64), l2 = __shfl_xor(l, o, 64);
+    const float mx = fmaxf(m, m2), use = mx == -INFINITY ? 0.f : mx;
+    const float wa = __builtin_amdgcn_exp2f(m - use), wb = __builtin_amdgcn_exp2f(m2 - use);
+    l = l * wa + l2 * wb;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor(acc[j], o, 64);
+    for (int j = 0; j < 4; ++j) acc[j] = acc[j] * wa + __shfl_xor(acc[j], o, 64) * wb;
+    m = mx;
   }
-  if (!live || mg != 0) return;
-  const bool none = m == -INFINITY && l == 0.f;
-  const f32x4 v = none ? f32x4{0.f, 0.f, 0.f, 0.f} : acc * (1.f / l);
-  *reinterpret_cast<uint2*>(p.o + (int64_t)t * p.orr + h * p.oh + d) =
-      uint2{pack16<F16>(v[0], v[1]), pack16<F16>(v[2], v[3])};
-  if (p.lse && d == 0) p.lse[(int64_t)h * p.new_rows + t] = none ? -INFINITY : (m_use + __log2f(l)) * LN2;
+  if (g != 0) return;
+  const float inv = n > 0 ? 1.f / l : 0.f;
+  *reinterpret_cast<uint2*>(p.o + (int64_t)tok * p.orr + head * p.oh + d) =
+      uint2{pack16<F16>(acc[0] * inv, acc[1] * inv), pack16<F16>(acc[2] * inv, acc[3] * inv)};
+  if (p.lse && d == 0)
+    p.lse[(int64_t)head * p.new_rows + tok] = n > 0 ? ((m == -INFINITY ? 0.f : m) + __log2f(l)) * LN2 : -INFINITY;
+}
+
+// The split tasks of the chunk kernel: blockIdx.x = task, blockIdx.y = 4 of its 128 rows
+template <bool F16>
+__global__ void __launch_bounds__(NT) attn_paged_merge_chunk(PagedArgs p) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int j = blockIdx.x, r = blockIdx.y * 4 + wave;
+  int hk, tile;
+  task_coords(p, p.whole + j, hk, tile);
+  const RowTile rt = find_tile(p, tile, lane);
+  if (rt.seq < 0) return;
+  const int len = checked_len(p.kv_lens[rt.seq], p.cap, p.fault);
+  const int t0 = rt.tile * p.per_tile;
+  const int t = r / p.group;
+  if (t >= min(p.per_tile, rt.nq - t0)) return;
+  const int limit = key_limit(len - rt.nq + t0 + t, len, p.block);
+  merge_row<F16, QB>(p, (int64_t)j * p.splits * QB + r, (limit + p.chunk - 1) / p.chunk, rt.c0 + t0 + t,
+                     hk * p.group + r - t * p.group, lane);
+}
+
+// The step kernel's rows: blockIdx.x = (sequence, K/V head), blockIdx.y = 4 of its rows
+template <bool F16, int RB>
+__global__ void __launch_bounds__(NT) attn_paged_merge_step(PagedArgs p) {
+  constexpr int RS = RB * 16;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = blockIdx.x / p.kv_heads, hk = blockIdx.x - b * p.kv_heads, r = blockIdx.y * 4 + wave;
+  const int c0 = p.cu[b];
+  const int nq = new_tokens(p, c0, p.cu[b + 1]);
+  if (r >= nq * p.group) return;
+  const int len = checked_len(p.kv_lens[b], p.cap, p.fault);
+  const int t = r / p.group;
+  const int limit = key_limit(len - nq + t, len, p.block);
+  merge_row<F16, RS>(p, (int64_t)blockIdx.x * p.splits * RS + r, (limit + p.chunk - 1) / p.chunk, c0 + t,
+                     hk * p.group + r - t * p.group, lane);
 }
 
 // ------------------------------------------------------------------------------------------------ plan
 struct Plan {
-  int rb;       // row blocks of the step kernel (0: the chunk kernel)
+  int rb;  // row blocks of the step kernel (0: the chunk kernel)
   int tiles, per_tile;
-  int splits, chunk;
-  int64_t ws;   // bytes of the partials
+  int whole, splits, chunk;
+  int64_t slots;  // workgroups that leave partials
+  int64_t ws;     // bytes of the partials
 };
 
 int cu_count() {
@@ -847,14 +923,15 @@ int cu_count() {
   return cache[dev] = cus;
 }
 
-// Key ranges: n of them cost ceil(workgroups * n / slots) rounds of (tiles / n + fixed) tile times each; the n with the
-// least cost, where a round's fixed part (prologue, partial rows, their merge) is worth `fixed` tiles.
-int best_splits(int64_t wgs, int tiles, int slots, double fixed, int most) {
+// Key ranges per task when all tasks are alike (one sequence): n of them cost ceil(tasks n / slots) rounds of
+// (tiles / n + fixed) tile times each, where a workgroup's fixed part (prologue, partial rows, their merge) is worth
+// `fixed` tiles; the n with the least cost.
+int even_splits(int64_t tasks, int tiles, int slots, double fixed, int most) {
   int best = 1;
   double cost = 0;
   for (int n = 1; n <= most && n <= tiles; ++n) {
-    const int64_t rounds = (wgs * n + slots - 1) / slots;
-    const double c = (double)rounds * ((tiles + n - 1) / n + fixed + (n > 1 ? 1.0 : 0.0));
+    const int64_t rounds = (tasks * n + slots - 1) / slots;
+    const double c = (double)rounds * ((tiles + n - 1) / n + (n > 1 ? fixed : 0.0));
     if (n == 1 || c < cost * 0.98) {
       best = n;
       cost = c;
@@ -862,37 +939,60 @@ int best_splits(int64_t wgs, int tiles, int slots, double fixed, int most) {
   }
   return best;
 }
+// ... when the sequences' lengths may differ (the host knows the longest only): the last workgroup to start ends
+// one range after the others, so the time is about tasks (tiles + n fixed) / slots + (tiles / n + fixed), least at
+// n = sqrt(tiles slots / (tasks fixed)).
+int ragged_splits(int64_t tasks, int tiles, int slots, double fixed, int most) {
+  const double n = std::sqrt((double)tiles * slots / ((double)tasks * fixed));
+  return std::max(1, std::min({most, tiles, (int)(n + 0.5)}));
+}
 
 Plan make_plan(const mapa_attn_paged_desc& d) {
   Plan pl = {};
   const int group = d.heads / d.cache.heads;
   const int cap = kv_cap(d.cache, d.batch);
   const int64_t rows = (int64_t)d.batch.max_new * group;
-  const int slots = 2 * cu_count();
+  const int slots = 2 * cu_count();  // resident workgroups
   int unit, tiles_k;
-  int64_t wgs;
+  int64_t tasks;
   if (rows <= 32) {
     pl.rb = rows <= 16 ? 1 : 2;
-    wgs = (int64_t)d.batch.seqs * d.cache.heads;
+    tasks = (int64_t)d.batch.seqs * d.cache.heads;
     unit = 4 * ST;
-    tiles_k = (cap + unit - 1) / unit;
-    pl.splits = best_splits(wgs, tiles_k, slots, 4.0, 128);
+    tiles_k = std::max(1, (cap + unit - 1) / unit);
+    pl.splits = d.batch.seqs == 1 ? even_splits(tasks, tiles_k, slots, 4.0, 128)
+                                  : ragged_splits(tasks, tiles_k, slots, 4.0, 128);
   } else {
     pl.per_tile = std::max(1, QB / group);
     const int64_t a = (int64_t)d.batch.new_rows / pl.per_tile + d.batch.seqs;
     const int64_t b = (int64_t)d.batch.seqs * ((d.batch.max_new + pl.per_tile - 1) / pl.per_tile);
     pl.tiles = (int)std::min(a, b);
-    wgs = (int64_t)pl.tiles * d.cache.heads;
+    tasks = (int64_t)pl.tiles * d.cache.heads;
     unit = KT;
-    tiles_k = (cap + unit - 1) / unit;
-    pl.splits = best_splits(wgs, tiles_k, slots, 3.0, 64);
+    tiles_k = std::max(1, (cap + unit - 1) / unit);
+    if (d.batch.seqs == 1) {  // full rounds of whole tasks, the rest cut so that it fills the chip too
+      pl.whole = (int)(tasks / slots * slots);
+      const int64_t rest = tasks - pl.whole;
+      pl.splits = rest ? even_splits(rest, tiles_k, slots, 4.0, 64) : 1;
+      if (pl.splits == 1) pl.whole = (int)tasks;
+    } else {
+      pl.splits = ragged_splits(tasks, tiles_k, slots, 4.0, 64);
+      if (pl.splits == 1) pl.whole = (int)tasks;
+    }
   }
-  tiles_k = std::max(tiles_k, 1);
   const int per = (tiles_k + pl.splits - 1) / pl.splits;
   pl.splits = (tiles_k + per - 1) / per;
   pl.chunk = per * unit;
-  pl.ws = pl.splits > 1 ? (int64_t)pl.splits * d.batch.new_rows * d.heads * (HD + 1) * 4 : 0;
+  pl.slots = pl.splits > 1 ? (tasks - pl.whole) * pl.splits : 0;
+  pl.ws = pl.slots * (pl.rb ? 16 * pl.rb : QB) * (HD + 1) * 4;
   return pl;
+}
+// the same work without a workspace: every task walks all its keys
+void unsplit(Plan& pl, const mapa_attn_paged_desc& d) {
+  pl.splits = 1;
+  pl.chunk = 1 << 30;
+  pl.whole = pl.rb ? 0 : pl.tiles * d.cache.heads;
+  pl.slots = pl.ws = 0;
 }
 
 int check_desc(const mapa_attn_paged_desc* d) {
@@ -912,15 +1012,28 @@ int check_desc(const mapa_attn_paged_desc* d) {
 }
 
 template <bool F16, int CK>
-void launch(const PagedArgs& a, const Plan& pl, hipStream_t stream) {
+void launch(const PagedArgs& a, const Plan& pl, unsigned grid, hipStream_t stream) {
+  if (pl.rb == 0) hipLaunchKernelGGL((attn_paged_chunk<F16, CK>), dim3(grid), dim3(NT), 0, stream, a);
+  else if (pl.rb == 1) hipLaunchKernelGGL((attn_paged_step<F16, CK, 1>), dim3(grid), dim3(NT), 0, stream, a);
+  else hipLaunchKernelGGL((attn_paged_step<F16, CK, 2>), dim3(grid), dim3(NT), 0, stream, a);
+}
+template <bool F16>
+int launch_all(const PagedArgs& a, const Plan& pl, int page_dtype, int64_t wgs, hipStream_t stream) {
+  if (page_dtype == MAPA_FP8) launch<F16, 1>(a, pl, (unsigned)wgs, stream);
+  else if (page_dtype == MAPA_I8) launch<F16, 2>(a, pl, (unsigned)wgs, stream);
+  else launch<F16, 0>(a, pl, (unsigned)wgs, stream);
+  MAPA_CHECK_LAUNCH("mapa_attention_paged");
+  if (pl.slots == 0) return 0;
   if (pl.rb == 0) {
-    const dim3 grid((unsigned)((int64_t)a.tiles * a.splits * a.kv_heads));
-    hipLaunchKernelGGL((attn_paged_chunk<F16, CK>), grid, dim3(NT), 0, stream, a);
+    const dim3 grid(a.tiles * a.kv_heads - a.whole, QB / 4);
+    hipLaunchKernelGGL((attn_paged_merge_chunk<F16>), grid, dim3(NT), 0, stream, a);
   } else {
-    const dim3 grid((unsigned)((int64_t)a.seqs * a.splits * a.kv_heads));
-    if (pl.rb == 1) hipLaunchKernelGGL((attn_paged_step<F16, CK, 1>), grid, dim3(NT), 0, stream, a);
-    else hipLaunchKernelGGL((attn_paged_step<F16, CK, 2>), grid, dim3(NT), 0, stream, a);
+    const dim3 grid(a.seqs * a.kv_heads, (std::min(a.max_new * a.group, 16 * pl.rb) + 3) / 4);
+    if (pl.rb == 1) hipLaunchKernelGGL((attn_paged_merge_step<F16, 1>), grid, dim3(NT), 0, stream, a);
+    else hipLaunchKernelGGL((attn_paged_merge_step<F16, 2>), grid, dim3(NT), 0, stream, a);
   }
+  MAPA_CHECK_LAUNCH("mapa_attention_paged (merge)");
+  return 0;
 }
 
 }  // namespace
@@ -938,11 +1051,7 @@ extern "C" int mapa_attention_paged(const mapa_attn_paged_desc* d, hipStream_t s
                      d->q_hstride % 8 == 0 && d->o_rstride % 8 == 0 && d->o_hstride % 8 == 0,
                  "mapa_attention_paged: query / output bases and strides must keep 16-byte alignment");
   Plan pl = make_plan(*d);
-  if (pl.splits > 1 && !(d->workspace && (uintptr_t)d->workspace % 16 == 0 && d->workspace_bytes >= pl.ws)) {
-    const int unit = pl.rb ? 4 * ST : KT;
-    pl.chunk = std::max(1, (kv_cap(d->cache, b) + unit - 1) / unit) * unit;
-    pl.splits = 1;
-  }
+  if (pl.ws && !(d->workspace && (uintptr_t)d->workspace % 16 == 0 && d->workspace_bytes >= pl.ws)) unsplit(pl, *d);
   PagedArgs a = {};
   a.page[0] = (const char*)d->cache.k; a.page[1] = (const char*)d->cache.v;
   a.exp[0] = d->cache.k_exp; a.exp[1] = d->cache.v_exp;
@@ -956,35 +1065,14 @@ extern "C" int mapa_attention_paged(const mapa_attn_paged_desc* d, hipStream_t s
   a.num_pages = d->cache.num_pages; a.psl = log2_of(d->cache.page_size);
   a.heads = d->heads; a.kv_heads = d->cache.heads; a.group = d->heads / d->cache.heads;
   a.block = d->mask_block;
-  a.splits = pl.splits; a.chunk = pl.chunk; a.tiles = pl.tiles; a.per_tile = pl.per_tile;
-  const int64_t wgs = (pl.rb ? (int64_t)b.seqs : (int64_t)pl.tiles) * a.splits * a.kv_heads;
-  MAPA_CHECK_ARG(wgs <= 0x7fffffff, "mapa_attention_paged: too many workgroups");
-  if (a.splits > 1) {
+  a.splits = pl.splits; a.chunk = pl.chunk; a.whole = pl.whole; a.tiles = pl.tiles; a.per_tile = pl.per_tile;
+  const int64_t wgs = pl.rb ? (int64_t)b.seqs * a.kv_heads * a.splits : pl.whole + pl.slots;
+  MAPA_CHECK_ARG(wgs <= 0x7fffffff && (int64_t)pl.tiles * a.kv_heads <= 0x7fffffff,
+                 "mapa_attention_paged: too many workgroups");
+  if (pl.slots) {
     a.part_o = (float*)d->workspace;
-    a.part_lse = a.part_o + (int64_t)a.splits * b.new_rows * a.heads * HD;
+    a.part_lse = a.part_o + pl.slots * (pl.rb ? 16 * pl.rb : QB) * HD;
   }
-  const int ck = d->cache.dtype == MAPA_FP8 ? 1 : d->cache.dtype == MAPA_I8 ? 2 : 0;
-  const bool f16 = d->dtype == MAPA_F16;
-  if (f16) {
-    if (ck == 0) launch<true, 0>(a, pl, stream);
-    else if (ck == 1) launch<true, 1>(a, pl, stream);
-    else launch<true, 2>(a, pl, stream);
-  } else {
-    if (ck == 0) launch<false, 0>(a, pl, stream);
-    else if (ck == 1) launch<false, 1>(a, pl, stream);
-    else launch<false, 2>(a, pl, stream);
-  }
-  MAPA_CHECK_LAUNCH("mapa_attention_paged");
-  if (a.splits > 1) {
-    const int64_t rows = (int64_t)b.new_rows * a.heads;
-    const int mg = a.splits >= 8 ? 4 : 1;
-    const int64_t per = NT / (16 * mg);
-    const dim3 grid((unsigned)((rows + per - 1) / per));
-    if (f16 && mg == 4) hipLaunchKernelGGL((attn_paged_merge<true, 4>), grid, dim3(NT), 0, stream, a);
-    else if (f16) hipLaunchKernelGGL((attn_paged_merge<true, 1>), grid, dim3(NT), 0, stream, a);
-    else if (mg == 4) hipLaunchKernelGGL((attn_paged_merge<false, 4>), grid, dim3(NT), 0, stream, a);
-    else hipLaunchKernelGGL((attn_paged_merge<false, 1>), grid, dim3(NT), 0, stream, a);
-    MAPA_CHECK_LAUNCH("mapa_attention_paged (merge)");
-  }
-  return 0;
+  return d->dtype == MAPA_F16 ? launch_all<true>(a, pl, d->cache.dtype, wgs, stream)
+                              : launch_all<false>(a, pl, d->cache.dtype, wgs, stream);
 }
