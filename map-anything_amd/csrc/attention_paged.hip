@@ -93,13 +93,37 @@ __device__ __forceinline__ int load_window(const PagedArgs& p, const int32_t* ro
   return v;
 }
 
-// 8 codes -> 8 operand words of the query's type, times the row's power of two (exact unless it leaves the type)
+template <bool F16>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if constexpr (F16) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, h2{(_Float16)a, (_Float16)b});  // v_cvt_pk_f16_f32
+  } else {
+    return pack_bf16x2(a, b);
+  }
+}
+
+// 8 codes -> 8 operand words of the query's type, times the row's power of two s (exact unless it leaves the type);
+// e4m3 pairs have an instruction that scales as it converts
 template <bool F16, bool I8>
 __device__ __forceinline__ bf16x8 decode8(uint2 w, float s) {
-  const f32x4 a = decode4<I8>(w.x, s), b = decode4<I8>(w.y, s);
-  const uint4 u = {pack_lp2(F16, a[0], a[1]), pack_lp2(F16, a[2], a[3]), pack_lp2(F16, b[0], b[1]),
-                   pack_lp2(F16, b[2], b[3])};
-  return __builtin_bit_cast(bf16x8, u);
+  if constexpr (I8) {
+    const f32x4 a = decode4<true>(w.x, s), b = decode4<true>(w.y, s);
+    return __builtin_bit_cast(bf16x8, uint4{pack16<F16>(a[0], a[1]), pack16<F16>(a[2], a[3]), pack16<F16>(b[0], b[1]),
+                                            pack16<F16>(b[2], b[3])});
+  } else if constexpr (F16) {
+    return __builtin_bit_cast(
+        bf16x8, uint4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.x, s, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.x, s, true)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.y, s, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w.y, s, true))});
+  } else {
+    return __builtin_bit_cast(
+        bf16x8, uint4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, s, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.x, s, true)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, s, false)),
+                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w.y, s, true))});
+  }
 }
 
 // whether any of 8 operand words is an infinity or a NaN
@@ -124,10 +148,6 @@ __device__ __forceinline__ bf16x8 only(bf16x8 v, int j) {
   return __builtin_bit_cast(bf16x8, r);
 }
 
-template <bool F16>
-__device__ __forceinline__ uint32_t pack16(float a, float b) {
-  return pack_lp2(F16, a, b);
-}
 // Row tile of the chunk kernel -> (sequence, its first packed row, its new tokens, tile in it), by a wave-wide prefix sum
 // over the sequences' tile counts, 64 at a time; seq -1: no such tile.
 struct RowTile {
@@ -176,16 +196,20 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hl = lane >> 5, l32 = lane & 31;
 
-  // whole tasks first, each XCD a contiguous run of them; then the split ones, range-major, so that workgroups which
-  // share a K/V range run together on one XCD
+  // whole tasks first, each XCD a contiguous run of them; then the split ones, where workgroups that share a K/V range
+  // run together on one XCD: (head, range, row tile) if all tasks are split — ranges outermost would give one XCD the
+  // last ranges, which only the longest sequence has (ragged causal chunks: 201 us so, 128 us head by head) — and
+  // (range, task) for the rest of one sequence's tasks
   int task, split = 0, slot = -1;
   if ((int)blockIdx.x < p.whole) {
     task = mapa_idx::xcd_remap(blockIdx.x, p.whole);
   } else {
     const int rest = p.tiles * p.kv_heads - p.whole;
     const int v = mapa_idx::xcd_remap(blockIdx.x - p.whole, rest * p.splits);
-    split = v / rest;
-    const int j = v - split * rest;
+    const int per = p.whole ? rest : p.tiles;
+    const int group = v / (per * p.splits), in = v - group * per * p.splits;
+    split = in / per;
+    const int j = group * per + in - split * per;
     task = p.whole + j;
     slot = j * p.splits + split;
   }
@@ -272,37 +296,45 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
       }
     }
   };
-  // 8-bit pages: thread -> tile row tid / 4, 16 codes; loaded one tile ahead, decoded after the tile's products
-  uint4 creg[2] = {};
-  uint32_t ereg[2] = {};
-  bool cin = false;
-  auto load8 = [&](int kt) __attribute__((always_inline)) {
+  // 8-bit pages: thread -> tile row tid / 4, 16 codes; loaded two tiles ahead (one set per tile parity), decoded after
+  // the products of the tile before
+  uint4 creg[2][2] = {};
+  uint32_t ereg[2][2] = {};
+  auto load8 = [&](int kt, auto set_tag) __attribute__((always_inline)) {
+    constexpr int set = decltype(set_tag)::value;
     const int key0 = kt * KT;
     need_window(key0);
     const int64_t at = cache_row(key0 + wave * 16);  // scalar; 16 rows of 64 B are contiguous
-    cin = key0 + (tid >> 2) < len;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      creg[x] = reinterpret_cast<const uint4*>(p.page[x] + at * 64)[lane];
-      ereg[x] = (p.exp[x] + at)[lane >> 2];
+      creg[set][x] = reinterpret_cast<const uint4*>(p.page[x] + at * 64)[lane];
+      ereg[set][x] = (p.exp[x] + at)[lane >> 2];
     }
   };
-  auto store8 = [&](int slot) __attribute__((always_inline)) {
-    char* dst = lds + slot * 2 * TILE;
+  auto store8 = [&](int kt, auto set_tag) __attribute__((always_inline)) {
+    constexpr int set = decltype(set_tag)::value;
+    char* dst = lds + set * 2 * TILE;
     const int row = tid >> 2, ch = (lane & 3) * 2;
+    const bool in = kt * KT + row < len;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
-      const float s = exponent_value(ereg[x]);
-      bf16x8 lo = decode8<F16, CK == 2>(uint2{creg[x].x, creg[x].y}, s);
-      bf16x8 hi = decode8<F16, CK == 2>(uint2{creg[x].z, creg[x].w}, s);
-      if (!cin) lo = hi = bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
+      const float s = exponent_value(ereg[set][x]);
+      bf16x8 lo = decode8<F16, CK == 2>(uint2{creg[set][x].x, creg[set][x].y}, s);
+      bf16x8 hi = decode8<F16, CK == 2>(uint2{creg[set][x].z, creg[set][x].w}, s);
+      if (!in) lo = hi = bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
       const int sw = x == 0 ? (row >> 1) & 7 : ((row >> 1) & 1) << 2;
       *reinterpret_cast<bf16x8*>(dst + x * TILE + row * 128 + ((ch ^ sw) << 4)) = lo;
       *reinterpret_cast<bf16x8*>(dst + x * TILE + row * 128 + (((ch + 1) ^ sw) << 4)) = hi;
     }
   };
-  if constexpr (CK == 0) stage16(0, kt0);
-  else load8(kt0);
+  using S0 = std::integral_constant<int, 0>;
+  using S1 = std::integral_constant<int, 1>;
+  if constexpr (CK == 0) {
+    stage16(0, kt0);
+  } else {
+    load8(kt0, S0());
+    if (kt0 + 1 < kt1) load8(kt0 + 1, S1());
+  }
 
   bf16x8 qf[4];
   {
@@ -310,7 +342,7 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) qf[kk] = *reinterpret_cast<const bf16x8*>(q + kk * 16 + 8 * hl);
   }
-  if constexpr (CK != 0) store8(0);
+  if constexpr (CK != 0) store8(kt0, S0());
 
   f32x16 o[2];
 #pragma unroll
@@ -362,9 +394,10 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
           }
       }
     }
-    if (kt + 1 < kt1) {
-      if constexpr (CK == 0) stage16(cur ^ 1, kt + 1);
-      else load8(kt + 1);
+    if constexpr (CK == 0) {
+      if (kt + 1 < kt1) stage16(cur ^ 1, kt + 1);
+    } else {
+      if (kt + 2 < kt1) load8(kt + 2, slot_tag);
     }
     if constexpr (MASK) {
 #pragma unroll
@@ -467,15 +500,13 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
           for (int s = 0; s < 2; ++s) o[dt] = mfma32x32x16<F16>(vf[dt][kb][s], pf[kb][s], o[dt]);
     }
     if constexpr (CK != 0) {
-      if (kt + 1 < kt1) store8(cur ^ 1);
+      if (kt + 1 < kt1) store8(kt + 1, std::integral_constant<int, cur ^ 1>());
     }
     __syncthreads();
   };
 
   using T_ = std::integral_constant<bool, true>;
   using F_ = std::integral_constant<bool, false>;
-  using S0 = std::integral_constant<int, 0>;
-  using S1 = std::integral_constant<int, 1>;
   __syncthreads();
   int kt = kt0;
   if (kt < kt_free) tile_step(kt, T_(), F_(), S0());
