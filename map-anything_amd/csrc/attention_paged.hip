@@ -61,6 +61,17 @@ typedef short s4v __attribute__((ext_vector_type(4)));
 typedef short s8v __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 
+typedef int i4v __attribute__((ext_vector_type(4)));
+
+// 16 B per lane from a buffer into LDS at lds + 16 lane, lanes past the buffer's end as zeros.  In asm so that the
+// compiler, which takes any LDS-DMA in flight for a writer of what a transposed LDS read reads, does not wait for it
+// there: it has no register output, and its completion is waited for by hand before the barrier that precedes the reads.
+// The five wait states before the load cover an operand SGPR that a vector instruction wrote just before (and M0).
+__device__ __forceinline__ void lds_dma16(i4v rsrc, int voffset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+               :: "v"(voffset), "s"(rsrc), "s"(lds) : "memory", "m0");
+}
+
 __device__ __forceinline__ s4v tr_read(const char* p) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)(p));
 }
@@ -192,7 +203,7 @@ __device__ __forceinline__ void task_coords(const PagedArgs& p, int task, int& h
 template <bool F16, int CK>
 __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
   constexpr int TILE = KT * 128;  // 64 rows x 128 B
-  __shared__ __attribute__((aligned(1024))) char lds[2 * 2 * TILE];
+  __shared__ __attribute__((aligned(1024))) char lds[2 * 2 * TILE];  // K by tile parity, then V
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hl = lane >> 5, l32 = lane & 31;
 
@@ -250,90 +261,109 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
   const int pages = (len + (1 << p.psl) - 1) >> p.psl;
   const int pmask = (1 << p.psl) - 1;
   const int64_t page_rows = (int64_t)p.kv_heads << p.psl, head_rows = (int64_t)hk << p.psl;
+  // Lane i holds the cache row at which (this head's part of) the sequence's page w0 + i begins, so that a tile's place
+  // is two v_readlanes and an addition away from being scalar; the next 64 pages are fetched when a tile passes them.
   int w0 = k_begin >> p.psl;
-  int win = load_window(p, trow, w0, pages, lane);
-  // row of the cache (head hk) of a 16-row-aligned key; keys past the last page: the last page (their rows are masked)
+  int64_t win;
+  auto fetch_window = [&]() __attribute__((always_inline)) {
+    win = (int64_t)load_window(p, trow, w0, pages, lane) * page_rows + head_rows;
+  };
+  fetch_window();
+  // row of the cache of a 16-row-aligned key; keys past the last page: the last page (their rows are hidden)
   auto cache_row = [&](int key) __attribute__((always_inline)) {
-    const int lp = min(key >> p.psl, pages - 1);
-    const int page = __builtin_amdgcn_readlane(win, lp - w0);
-    return (int64_t)page * page_rows + head_rows + (key & pmask);
+    const int i = min(key >> p.psl, pages - 1) - w0;
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)win, i);
+    const int hi = __builtin_amdgcn_readlane((int)(win >> 32), i);
+    return (int64_t)(((uint64_t)(uint32_t)hi << 32) | lo) + (key & pmask);
   };
   auto need_window = [&](int key0) __attribute__((always_inline)) {  // pages of keys [key0, key0 + 64) in the window
     const int last = min((key0 + KT - 1) >> p.psl, pages - 1);
-    if (last - w0 >= 64) {
+    if (__builtin_expect(last - w0 >= 64, 0)) {
       w0 = key0 >> p.psl;
-      win = load_window(p, trow, w0, pages, lane);
+      fetch_window();
     }
   };
 
-  const char* zero = reinterpret_cast<const char*>(g_mapa_zero_page);
-  // 16-bit pages: 16 pieces of 8 rows x 128 B (K: 0..7, V: 8..15), four per wave; the 16-B column is XOR-swizzled on
-  // the source so that the LDS image stays lane-linear.  A piece lies in one page: a scalar base and a fixed offset per
-  // lane, but for the tile that the sequence ends in, whose rows past the end come from the zero page.
+  // Staging.  A tile's K is needed one step before its V, so step t brings K of tile t + 2 and V of tile t; the V rows'
+  // place in the cache is K's of two steps ago (`at`, by tile parity).  Tile numbers past the range are clamped: what
+  // they bring is not used.
+  //  * 16-bit pages: a wave moves rows 8 wave and 32 + 8 wave .. + 7 of the tile (8 rows x 128 B lie in one page: a
+  //    scalar base and a fixed offset per lane), the 16-B column XOR-swizzled on the source so that the LDS image stays
+  //    lane-linear.  V's buffer ends where the sequence does, so that rows past it arrive as zeros: whatever their memory
+  //    holds must not meet a zero probability (hidden scores are replaced, so K needs no such care).
+  //  * 8-bit pages: thread -> tile row tid / 4, 16 codes, fetched a step earlier and decoded on the way into LDS.
+  constexpr int NA = CK == 0 ? 2 : 1;  // cache rows to remember per tile
+  int64_t at[2][NA];
   const int prow8 = lane >> 3;
   const int koff = prow8 * 128 + (((lane & 7) ^ (((wave & 1) * 4 + (lane >> 4)) & 7)) << 4);
   const int voff = prow8 * 128 + (((lane & 7) ^ (((lane >> 4) & 1) << 2)) << 4);
-  auto stage16 = [&](int slot_, int kt) __attribute__((always_inline)) {
-    char* dst = lds + slot_ * 2 * TILE;
+  auto place = [&](int kt, auto par_tag) __attribute__((always_inline)) {
+    constexpr int par = decltype(par_tag)::value;
     const int key0 = kt * KT;
     need_window(key0);
-    const bool full = key0 + KT <= len;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) at[par][i] = cache_row(key0 + (CK == 0 ? (i * 4 + wave) * 8 : wave * 16));
+  };
+  const uint32_t lds_base = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
+  auto dma = [&](auto x_tag, int kt, auto par_tag, auto full_tag) __attribute__((always_inline)) {  // x: 0 K, 1 V
+    constexpr int x = decltype(x_tag)::value, par = decltype(par_tag)::value;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int k8 = (i * 4 + wave) * 8;  // first tile row of the piece (K and V alike)
-      const int64_t at = cache_row(key0 + k8) * 128;
-      const char* kp = p.page[0] + at;
-      const char* vp = p.page[1] + at;
-      if (full) {
-        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void*)kp, 0, 1024, 0x00020000);
-        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void*)vp, 0, 1024, 0x00020000);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_ptr_t)(dst + k8 * 128), 16, koff, 0, 0, 0);
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_ptr_t)(dst + TILE + k8 * 128), 16, voff, 0, 0, 0);
-      } else {
-        const bool in = key0 + k8 + prow8 < len;
-        __builtin_amdgcn_global_load_lds(in ? kp + koff : zero, (lds_ptr_t)(dst + k8 * 128), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds(in ? vp + voff : zero, (lds_ptr_t)(dst + TILE + k8 * 128), 16, 0, 0);
+      const int k8 = (i * 4 + wave) * 8;
+      int bytes = 1024;
+      if constexpr (x == 1 && !decltype(full_tag)::value) {
+        const int rows_left = len - kt * KT - k8;
+        bytes = rows_left >= 8 ? 1024 : rows_left > 0 ? rows_left * 128 : 0;
       }
+      const uint64_t base = (uint64_t)(p.page[x] + at[par][i] * 128);
+      lds_dma16(i4v{(int)(uint32_t)base, (int)(base >> 32), bytes, 0x00020000}, x == 0 ? koff : voff,
+                lds_base + (2 * x + par) * TILE + k8 * 128);
     }
   };
-  // 8-bit pages: thread -> tile row tid / 4, 16 codes; loaded two tiles ahead (one set per tile parity), decoded after
-  // the products of the tile before
-  uint4 creg[2][2] = {};
-  uint32_t ereg[2][2] = {};
-  auto load8 = [&](int kt, auto set_tag) __attribute__((always_inline)) {
-    constexpr int set = decltype(set_tag)::value;
-    const int key0 = kt * KT;
-    need_window(key0);
-    const int64_t at = cache_row(key0 + wave * 16);  // scalar; 16 rows of 64 B are contiguous
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      creg[set][x] = reinterpret_cast<const uint4*>(p.page[x] + at * 64)[lane];
-      ereg[set][x] = (p.exp[x] + at)[lane >> 2];
-    }
+  uint4 creg[2] = {};
+  uint32_t ereg[2] = {};
+  auto fetch8 = [&](int x, auto par_tag) __attribute__((always_inline)) {
+    constexpr int par = decltype(par_tag)::value;
+    creg[x] = reinterpret_cast<const uint4*>(p.page[x] + at[par][0] * 64)[lane];
+    ereg[x] = (p.exp[x] + at[par][0])[lane >> 2];
   };
-  auto store8 = [&](int kt, auto set_tag) __attribute__((always_inline)) {
-    constexpr int set = decltype(set_tag)::value;
-    char* dst = lds + set * 2 * TILE;
+  auto store8 = [&](int x, int kt, auto par_tag) __attribute__((always_inline)) {
+    constexpr int par = decltype(par_tag)::value;
+    char* dst = lds + (2 * x + par) * TILE;
     const int row = tid >> 2, ch = (lane & 3) * 2;
-    const bool in = kt * KT + row < len;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const float s = exponent_value(ereg[set][x]);
-      bf16x8 lo = decode8<F16, CK == 2>(uint2{creg[set][x].x, creg[set][x].y}, s);
-      bf16x8 hi = decode8<F16, CK == 2>(uint2{creg[set][x].z, creg[set][x].w}, s);
-      if (!in) lo = hi = bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
-      const int sw = x == 0 ? (row >> 1) & 7 : ((row >> 1) & 1) << 2;
-      *reinterpret_cast<bf16x8*>(dst + x * TILE + row * 128 + ((ch ^ sw) << 4)) = lo;
-      *reinterpret_cast<bf16x8*>(dst + x * TILE + row * 128 + (((ch + 1) ^ sw) << 4)) = hi;
-    }
+    const float s = exponent_value(ereg[x]);
+    bf16x8 lo = decode8<F16, CK == 2>(uint2{creg[x].x, creg[x].y}, s);
+    bf16x8 hi = decode8<F16, CK == 2>(uint2{creg[x].z, creg[x].w}, s);
+    if (kt * KT + row >= len) lo = hi = bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    const int sw = x == 0 ? (row >> 1) & 7 : ((row >> 1) & 1) << 2;
+    *reinterpret_cast<bf16x8*>(dst + row * 128 + ((ch ^ sw) << 4)) = lo;
+    *reinterpret_cast<bf16x8*>(dst + row * 128 + (((ch + 1) ^ sw) << 4)) = hi;
   };
-  using S0 = std::integral_constant<int, 0>;
-  using S1 = std::integral_constant<int, 1>;
+  using T_ = std::integral_constant<bool, true>;
+  using F_ = std::integral_constant<bool, false>;
+  using P0 = std::integral_constant<int, 0>;
+  using P1 = std::integral_constant<int, 1>;
+  // the steps' barrier: this wave's DMA has landed and its LDS accesses are done
+  auto step_barrier = [&]() __attribute__((always_inline)) {
+    if constexpr (CK == 0) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  place(kt0, P0());
   if constexpr (CK == 0) {
-    stage16(0, kt0);
+    dma(P0(), kt0, P0(), F_());
+    place(min(kt0 + 1, kt1 - 1), P1());
+    dma(P0(), kt0 + 1, P1(), F_());
   } else {
-    load8(kt0, S0());
-    if (kt0 + 1 < kt1) load8(kt0 + 1, S1());
+    fetch8(0, P0());
+    store8(0, kt0, P0());
+    place(min(kt0 + 1, kt1 - 1), P1());
+    fetch8(0, P1());
+    fetch8(1, P0());
+    store8(0, kt0 + 1, P1());
+    place(min(kt0 + 2, kt1 - 1), P0());
+    fetch8(0, P0());
   }
 
   bf16x8 qf[4];
@@ -342,9 +372,9 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) qf[kk] = *reinterpret_cast<const bf16x8*>(q + kk * 16 + 8 * hl);
   }
-  if constexpr (CK != 0) store8(kt0, S0());
 
-  f32x16 o[2];
+  f32x16 o[2], st[2][2];  // output rows; scores by tile parity
+  bf16x8 pf[4];           // probabilities of the tile before, waiting for its V
 #pragma unroll
   for (int d = 0; d < 2; ++d)
 #pragma unroll
@@ -352,102 +382,160 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
   float m_ref = 0.f, l_run = 0.f;
   const float c = p.c;
 
-  // FIRST: the range's first tile (sets m_ref).  MASK: keys of the tile may be hidden from rows.  SLOT: LDS slot.
-  auto tile_step = [&](int kt, auto first_tag, auto mask_tag, auto slot_tag) __attribute__((always_inline)) {
-    constexpr bool FIRST = decltype(first_tag)::value;
-    constexpr bool MASK = decltype(mask_tag)::value;
-    constexpr int cur = decltype(slot_tag)::value;
-    const char* Ks = lds + cur * 2 * TILE;
-    const char* Vs = Ks + TILE;
-    bf16x8 kf[2][4];
+  // K fragment: keys 32 kb + l32, dims 16 kk + 8 hl ..; V^T fragment: dims 32 dt + l32, keys 16 f + 8 (j / 4) + 4 hl + j % 4
+  // (transposed LDS reads), the order in which the scores come out of K Q^T
+  auto k_frag = [&](const char* Ks, int kb, int kk) __attribute__((always_inline)) {
+    const int row = kb * 32 + l32;
+    return *reinterpret_cast<const bf16x8*>(Ks + row * 128 + (((kk * 2 + hl) ^ ((row >> 1) & 7)) << 4));
+  };
+  auto v_frag = [&](const char* Vs, int dt, int f) __attribute__((always_inline)) {
+    const int i4 = lane & 15, q4 = i4 >> 2, p4 = i4 & 3, grp = (lane >> 4) & 1;
+    const int cc = dt * 32 + 16 * grp + 4 * p4, ch = cc >> 3, within = (cc & 7) * 2;
+    const int R0 = 16 * f + 4 * hl + q4, R1 = R0 + 8;
+    const s4v lo = tr_read(Vs + R0 * 128 + ((ch ^ (((R0 >> 1) & 1) << 2)) << 4) + within);
+    const s4v hi = tr_read(Vs + R1 * 128 + ((ch ^ (((R1 >> 1) & 1) << 2)) << 4) + within);
+    return (bf16x8)s8v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  };
+  auto row_max = [&](const f32x16* s) __attribute__((always_inline)) {
+    float mx = s[0][0];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      const int row = kb * 32 + l32;
+    for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        kf[kb][kk] = *reinterpret_cast<const bf16x8*>(Ks + row * 128 + (((kk * 2 + hl) ^ ((row >> 1) & 7)) << 4));
-    }
-    f32x16 st[2];
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+    return fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * c;
+  };
+  auto hide = [&](f32x16* s, int kt) __attribute__((always_inline)) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
+    for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) st[kb][i] = 0.f;
+      for (int i = 0; i < 16; ++i) {
+        const int key = kt * KT + kb * 32 + (i & 3) + 8 * (i >> 2) + 4 * hl;
+        s[kb][i] = key < limit ? s[kb][i] : -INFINITY;
+      }
+  };
+  // O^T += V^T P^T of tile kt, with a look at V first: an infinity or NaN of a key that some rows do not see, times
+  // their zero probability, must not reach them — such a tile is added key by key, where it is seen
+  auto pv_checked = [&](const char* Vs, int kt) __attribute__((always_inline)) {
+    bf16x8 vf[2][4];
+    bool special = false;
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) st[kb] = mfma32x32x16<F16>(kf[kb][kk], qf[kk], st[kb]);
-    }
-    // V^T fragments (transposed LDS reads): every LDS read of the tile is issued before the next tile's DMA
-    bf16x8 vf[2][2][2];
-    {
-      const int i4 = lane & 15, q4 = i4 >> 2, p4 = i4 & 3, grp = (lane >> 4) & 1;
+    for (int f = 0; f < 4; ++f)
 #pragma unroll
       for (int dt = 0; dt < 2; ++dt) {
-        const int cc = dt * 32 + 16 * grp + 4 * p4;
-        const int ch = cc >> 3, within = (cc & 7) * 2;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const int R0 = kb * 32 + 16 * s + 4 * hl + q4, R1 = R0 + 8;
-            const s4v lo = tr_read(Vs + R0 * 128 + ((ch ^ (((R0 >> 1) & 1) << 2)) << 4) + within);
-            const s4v hi = tr_read(Vs + R1 * 128 + ((ch ^ (((R1 >> 1) & 1) << 2)) << 4) + within);
-            vf[dt][kb][s] = s8v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-          }
+        vf[dt][f] = v_frag(Vs, dt, f);
+        special |= any_special<F16>(vf[dt][f]);
       }
-    }
-    if constexpr (CK == 0) {
-      if (kt + 1 < kt1) stage16(cur ^ 1, kt + 1);
-    } else {
-      if (kt + 2 < kt1) load8(kt + 2, slot_tag);
-    }
-    if constexpr (MASK) {
+    if (__builtin_expect(__any(special), 0)) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int f = 0; f < 4; ++f)
+#pragma unroll 1
+        for (int jj = 0; jj < 16; ++jj) {
+          const int j = jj & 7, h2 = jj >> 3;
+          const int key = kt * KT + 16 * f + (j & 3) + 8 * (j >> 2) + 4 * h2;
+          const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+          const bf16x8 pk = hl == h2 ? only(pf[f], j) : z;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = kt * KT + kb * 32 + (i & 3) + 8 * (i >> 2) + 4 * hl;
-          st[kb][i] = key < limit ? st[kb][i] : -INFINITY;
-        }
-    }
-
-    bf16x8 pf[2][2];
-    float ls;
-    auto exp_pack = [&]() __attribute__((always_inline)) {
-      float a[4];  // four sums, seeded with the first values
-      const float nm = -m_ref;
+          for (int dt = 0; dt < 2; ++dt) {
+            const bf16x8 vk = hl == h2 ? only(vf[dt][f], j) : z;
+            f32x16 t;
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+            for (int i = 0; i < 16; ++i) t[i] = 0.f;
+            t = mfma32x32x16<F16>(vk, pk, t);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          uint32_t pk[4];
-#pragma unroll
-          for (int j = 0; j < 8; j += 2) {
-            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[kb][8 * s + j], c, nm));
-            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(st[kb][8 * s + j + 1], c, nm));
-            a[j & 3] = (kb == 0 && s == 0 && j < 4) ? e0 : a[j & 3] + e0;
-            a[(j + 1) & 3] = (kb == 0 && s == 0 && j < 4) ? e1 : a[(j + 1) & 3] + e1;
-            pk[j / 2] = pack16<F16>(e0, e1);
+            for (int i = 0; i < 16; ++i) o[dt][i] = key < limit ? o[dt][i] + t[i] : o[dt][i];
           }
-          pf[kb][s] = __builtin_bit_cast(bf16x8, uint4{pk[0], pk[1], pk[2], pk[3]});
         }
-      ls = (a[0] + a[1]) + (a[2] + a[3]);
-    };
-    auto row_max = [&]() __attribute__((always_inline)) {
-      float mx = st[0][0];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[kb][i]);
-      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-      return fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) * c;
-    };
-    if constexpr (FIRST) {
-      const float m = row_max();
-      m_ref = fmaxf(m, -1e38f);  // finite also for a row that sees none of the range
-      exp_pack();
     } else {
-      exp_pack();
+#pragma unroll
+      for (int f = 0; f < 4; ++f)
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt) o[dt] = mfma32x32x16<F16>(vf[dt][f], pf[f], o[dt]);
+    }
+  };
+
+  // Step t (parity PAR): the softmax of tile t's scores, the products K Q^T of tile t + 1 and V^T P^T of tile t - 1.
+  // The two MFMA chains and the softmax are independent, so the matrix unit runs under the exponentials: 16 MFMAs of 32
+  // cycles between 16 groups of two scores (2 fma, 2 exp, 2 add, 1 conversion: 36 cycles).
+  auto step = [&](int t, auto first_tag, auto mask_tag, auto par_tag) __attribute__((always_inline)) {
+    constexpr bool FIRST = decltype(first_tag)::value;
+    constexpr bool MASK = decltype(mask_tag)::value;
+    constexpr int par = decltype(par_tag)::value, nxt = par ^ 1;
+    using PN = std::integral_constant<int, nxt>;
+    f32x16(&s)[2] = st[par];
+    f32x16(&sn)[2] = st[nxt];
+    const char* Ks = lds + nxt * TILE;        // K of tile t + 1
+    const char* Vs = lds + (2 + nxt) * TILE;  // V of tile t - 1
+    constexpr bool PV = !MASK && !FIRST;
+    bf16x8 kf[2][2], vf[2][2];
+    auto frags = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        kf[i & 1][x] = k_frag(Ks, x, i);
+        if constexpr (PV) vf[i & 1][x] = v_frag(Vs, x, i);
+      }
+    };
+    frags(0);
+    if constexpr (CK == 0) {
+      dma(P1(), t, par_tag, std::integral_constant<bool, !MASK>());
+      place(min(t + 2, kt1 - 1), par_tag);
+      dma(P0(), t + 2, par_tag, F_());
+    } else {
+      store8(1, t, par_tag);
+      store8(0, t + 2, par_tag);
+      fetch8(1, PN());
+      place(min(t + 3, kt1 - 1), PN());
+      fetch8(0, PN());
+    }
+    if constexpr (MASK) hide(s, t);
+    if constexpr (FIRST) m_ref = fmaxf(row_max(s), -1e38f);  // finite also for a row that sees none of the range
+    const float nm = -m_ref;
+    if constexpr (MASK && !FIRST) pv_checked(Vs, t - 1);
+    // Group n: MFMA n; the exponents of scores 2n, 2n + 1; behind them the sums and the conversion of the two before,
+    // ahead the fma of the two after (an exponential's result is late).  Scores in register order: key block, then
+    // accumulator element, which is the order of P's fragments.
+    float a[4] = {0.f, 0.f, 0.f, 0.f}, x[2], e[2], y[2];
+    uint32_t pk[4];
+    x[0] = __builtin_fmaf(s[0][0], c, nm);
+    x[1] = __builtin_fmaf(s[0][1], c, nm);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int n = 0; n < 17; ++n) {
+      const int i = n >> 2, g = n & 3;
+      if (n < 16) {
+        if (g < 2) {
+          if (i == 0) {
+#pragma unroll
+            for (int z = 0; z < 16; ++z) sn[g][z] = 0.f;
+          }
+          sn[g] = mfma32x32x16<F16>(kf[i & 1][g], qf[i], sn[g]);
+        } else if constexpr (PV) {
+          o[g - 2] = mfma32x32x16<F16>(vf[i & 1][g - 2], pf[i], o[g - 2]);
+        }
+        if (g == 0 && i < 3) frags(i + 1);
+        e[0] = __builtin_amdgcn_exp2f(x[0]);
+        e[1] = __builtin_amdgcn_exp2f(x[1]);
+        if (n < 15) {
+          x[0] = __builtin_fmaf(s[(2 * n + 2) >> 4][(2 * n + 2) & 15], c, nm);
+          x[1] = __builtin_fmaf(s[(2 * n + 3) >> 4][(2 * n + 3) & 15], c, nm);
+        }
+      }
+      if (n > 0) {
+        const int b2 = 2 * ((n - 1) & 1);
+        a[b2] = n < 3 ? y[0] : a[b2] + y[0];
+        a[b2 + 1] = n < 3 ? y[1] : a[b2 + 1] + y[1];
+        pk[(n - 1) & 3] = pack16<F16>(y[0], y[1]);
+        asm volatile("" : "+v"(pk[(n - 1) & 3]));  // here, not sunk behind the check below
+        if (((n - 1) & 3) == 3) pf[(n - 1) >> 2] = __builtin_bit_cast(bf16x8, uint4{pk[0], pk[1], pk[2], pk[3]});
+      }
+      y[0] = e[0];
+      y[1] = e[1];
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    float ls = (a[0] + a[1]) + (a[2] + a[3]);
+    if constexpr (!FIRST) {
       if (__builtin_expect(__any(!(ls <= REBASE_SUM)), 0)) {  // NaN rebases too
-        const float m = fmaxf(row_max(), m_ref);
+        const float m = fmaxf(row_max(s), m_ref);
         const float alpha = __builtin_amdgcn_exp2f(m_ref - m);
         m_ref = m;
         l_run *= alpha;
@@ -455,74 +543,51 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
         for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
-        exp_pack();
+        ls = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t pk[4];
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int e = 8 * (i & 1) + 2 * g;
+            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 1][e], c, -m));
+            const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 1][e + 1], c, -m));
+            ls += e0 + e1;
+            pk[g] = pack16<F16>(e0, e1);
+          }
+          pf[i] = __builtin_bit_cast(bf16x8, uint4{pk[0], pk[1], pk[2], pk[3]});
+        }
       }
     }
     l_run += ls;
-    bool special = false;
-    if constexpr (MASK) {  // an infinity or NaN in V: zero times it must not reach the rows that do not see its key
-#pragma unroll
-      for (int dt = 0; dt < 2; ++dt)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int s = 0; s < 2; ++s) special |= any_special<F16>(vf[dt][kb][s]);
-      special = __any(special);
-    }
-    if (MASK && __builtin_expect(special, 0)) {
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll 1
-          for (int jj = 0; jj < 16; ++jj) {  // one key at a time, added where it is seen
-            const int j = jj & 7, h2 = jj >> 3;
-            const int key = kt * KT + kb * 32 + 16 * s + (j & 3) + 8 * (j >> 2) + 4 * h2;
-            const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
-            const bf16x8 pk = hl == h2 ? only(pf[kb][s], j) : z;
-#pragma unroll
-            for (int dt = 0; dt < 2; ++dt) {
-              const bf16x8 vk = hl == h2 ? only(vf[dt][kb][s], j) : z;
-              f32x16 t;
-#pragma unroll
-              for (int i = 0; i < 16; ++i) t[i] = 0.f;
-              t = mfma32x32x16<F16>(vk, pk, t);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) o[dt][i] = key < limit ? o[dt][i] + t[i] : o[dt][i];
-            }
-          }
-    } else {
-#pragma unroll
-      for (int dt = 0; dt < 2; ++dt)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int s = 0; s < 2; ++s) o[dt] = mfma32x32x16<F16>(vf[dt][kb][s], pf[kb][s], o[dt]);
-    }
-    if constexpr (CK != 0) {
-      if (kt + 1 < kt1) store8(kt + 1, std::integral_constant<int, cur ^ 1>());
-    }
-    __syncthreads();
+    step_barrier();
   };
 
-  using T_ = std::integral_constant<bool, true>;
-  using F_ = std::integral_constant<bool, false>;
-  __syncthreads();
+  step_barrier();
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) st[0][kb][i] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) st[0][kb] = mfma32x32x16<F16>(k_frag(lds, kb, kk), qf[kk], st[0][kb]);
+  }
+  step_barrier();  // K of the first tile is read: its slot is free
   int kt = kt0;
-  if (kt < kt_free) tile_step(kt, T_(), F_(), S0());
-  else tile_step(kt, T_(), T_(), S0());
+  if (kt < kt_free) step(kt, T_(), F_(), P0());
+  else step(kt, T_(), T_(), P0());
   ++kt;
 #pragma unroll 1
   for (; kt + 1 < kt_free; kt += 2) {
-    tile_step(kt, F_(), F_(), S1());
-    tile_step(kt + 1, F_(), F_(), S0());
+    step(kt, F_(), F_(), P1());
+    step(kt + 1, F_(), F_(), P0());
   }
   // the rest: at most one more free tile, then the masked ones (an extra mask on a free tile changes nothing)
 #pragma unroll 1
   for (; kt < kt1; kt += 2) {
-    tile_step(kt, F_(), T_(), S1());
-    if (kt + 1 < kt1) tile_step(kt + 1, F_(), T_(), S0());
+    step(kt, F_(), T_(), P1());
+    if (kt + 1 < kt1) step(kt + 1, F_(), T_(), P0());
   }
+  pv_checked(lds + (2 + ((kt1 - 1 - kt0) & 1)) * TILE, kt1 - 1);
 
   const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
   // a row that sees keys of the range has a sum of one at least, unless every score is -inf (then NaN, as the formula)
