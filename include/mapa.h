@@ -464,7 +464,7 @@ int mapa_rope2d(void* tokens, int dtype, int B, int H, int N, int D, int64_t sb,
 /* ---------------------------------------------------------------------------------------------------------
  * Rotary positions with several axes (time, row, column, ...): the general form of mapa_rope2d, out of place or in
  * place, forward and backward, one or two tensors (queries and keys) in one launch.
- * Tensor i (i < 2, x[i] may be NULL): x[i] -> y[i] (equal pointers AND strides: in place), shape (batch, heads[i],
+ * Tensor i (i < 2, x[i] may be NULL): x[i] -> y[i] (equal pointers AND strides: in place), shape (batch, heads[i] <= 2048,
  * tokens, head_dim), element strides (b, h, n), contiguous head dim.  section[a] pairs belong to axis a; with
  * S = sum(section), 2 S <= head_dim, the dims from 2 S on are copied.  Pair i (axis a, its j-th pair) turns by
  * positions[b][n][a] * freq[i] radians (the angle is reduced in 64 bits): u' = u cos - v sin, v' = v cos + u sin;
@@ -502,7 +502,7 @@ int mapa_rope_axes(const mapa_rope_axes_desc* d, mapa_stream_t stream);
  * MAPA_I8 codes with exponent bytes k_exp / v_exp [num_pages][heads][page_size]: value = code * 2^(byte - 127), byte
  * the least with max|row| <= 448 (127) * 2^(byte - 127), taken of max(max|row|, 2^-100).  A power of two makes the scaling exact, so a
  * value is rounded once, at the store (to nearest even).  A row with a value that is not finite is held as NaN.
- * page_size: a power of two, 16 .. 1024.
+ * page_size: a power of two, 16 .. 1024; heads: 2048 at most.
  * mapa_kv_batch: `seqs` sequences; token position p of sequence b lives in page table[b * table_stride + p /
  * page_size], row p % page_size.  kv_lens[b]: tokens in the cache, the new ones included; the new tokens of sequence b
  * are the packed rows cu_new[b] .. cu_new[b + 1] - 1 and hold its last positions.  Rows from cu_new[seqs] to

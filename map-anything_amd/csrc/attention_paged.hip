@@ -66,10 +66,11 @@ typedef int i4v __attribute__((ext_vector_type(4)));
 // 16 B per lane from a buffer into LDS at lds + 16 lane, lanes past the buffer's end as zeros.  In asm so that the
 // compiler, which takes any LDS-DMA in flight for a writer of what a transposed LDS read reads, does not wait for it
 // there: it has no register output, and its completion is waited for by hand before the barrier that precedes the reads.
-// The five wait states before the load cover an operand SGPR that a vector instruction wrote just before (and M0).
+// The five wait states before the load cover an operand SGPR that a vector instruction wrote just before (and M0, which
+// nothing else in these kernels uses).
 __device__ __forceinline__ void lds_dma16(i4v rsrc, int voffset, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
-               :: "v"(voffset), "s"(rsrc), "s"(lds) : "memory", "m0");
+               :: "v"(voffset), "s"(rsrc), "s"(lds) : "memory");
 }
 
 __device__ __forceinline__ s4v tr_read(const char* p) {
@@ -236,6 +237,7 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
   const int pos0 = len - nq + t0;                         // position of the first token
   const int lim_lo = key_limit(pos0, len, p.block);
   const int lim_hi = key_limit(pos0 + (rows - 1) / p.group, len, p.block);
+  if (lim_hi <= p.chunk && split == 0) slot = -1;  // one range holds all of the tile's keys: no partials
   const int k_begin = split * p.chunk, k_end = slot < 0 ? lim_hi : min(k_begin + p.chunk, lim_hi);
 
   // this lane's row
@@ -665,7 +667,7 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
     limit[rb] = key_limit(pos0 + rt, len, p.block);
   }
   if (k_begin >= k_end) {  // uniform: the whole workgroup leaves (the merge knows which ranges are empty)
-    for (int i = tid; p.splits == 1 && i < rows * 8; i += NT) {
+    for (int i = tid; split == 0 && i < rows * 8; i += NT) {
       const int r = i >> 3, rt = r / p.group, h = hk * p.group + r - rt * p.group, t = c0 + rt;
       reinterpret_cast<uint4*>(p.o + (int64_t)t * p.orr + h * p.oh)[i & 7] = uint4{0, 0, 0, 0};
       if (p.lse && (i & 7) == 0) p.lse[(int64_t)h * p.new_rows + t] = -INFINITY;
@@ -897,7 +899,7 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
     const float lse2 = !seen ? -INFINITY : l > 0.f ? m_use + __log2f(l) : __builtin_nanf("");
     f32x4 v = acc * inv;
     if (!seen) v = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (p.splits == 1) {
+    if (lim_hi <= p.chunk) {  // one range holds all keys: no partials
       *reinterpret_cast<uint2*>(p.o + (int64_t)t * p.orr + h * p.oh + d) =
           uint2{pack16<F16>(v[0], v[1]), pack16<F16>(v[2], v[3])};
       if (p.lse && d == 0) p.lse[(int64_t)h * p.new_rows + t] = lse2 * LN2;
@@ -910,6 +912,33 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
 }
 
 // ------------------------------------------------------------------------------------------------ merge
+// Eight ranges' partials (their log2 sums ls, normalised rows v) into the running maximum, weight and row
+__device__ __forceinline__ void merge_ranges(const float* ls, const f32x4* v, float& m, float& l, f32x4& acc) {
+  float mx = m;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) mx = fmaxf(mx, ls[i]);
+  const float use = mx == -INFINITY ? 0.f : mx;
+  const float keep = __builtin_amdgcn_exp2f(m - use);
+  l *= keep;
+  acc *= keep;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float w = __builtin_amdgcn_exp2f(ls[i] - use);
+    l += w;
+    acc += w * v[i];
+  }
+  m = mx;
+}
+template <bool F16>
+__device__ __forceinline__ void merge_store(const PagedArgs& p, int n, float m, float l, f32x4 acc, int tok, int head,
+                                            int d) {
+  const float inv = n > 0 ? 1.f / l : 0.f;
+  *reinterpret_cast<uint2*>(p.o + (int64_t)tok * p.orr + head * p.oh + d) =
+      uint2{pack16<F16>(acc[0] * inv, acc[1] * inv), pack16<F16>(acc[2] * inv, acc[3] * inv)};
+  if (p.lse && d == 0)
+    p.lse[(int64_t)head * p.new_rows + tok] = n > 0 ? ((m == -INFINITY ? 0.f : m) + __log2f(l)) * LN2 : -INFINITY;
+}
+
 // One wave per row: four groups of 16 lanes x 4 columns, group g over the key ranges g, g + 4, ...; 32 ranges' partials
 // are in flight at once, joined in a fixed order.  `first`: the row in its first range's slot, `n`: ranges with a key
 // that the row sees.
@@ -933,20 +962,7 @@ __device__ __forceinline__ void merge_row(const PagedArgs& p, int64_t first, int
         v[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * HD + d);
       }
     }
-    float mx = m;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) mx = fmaxf(mx, ls[i]);
-    const float use = mx == -INFINITY ? 0.f : mx;
-    const float keep = __builtin_amdgcn_exp2f(m - use);
-    l *= keep;
-    acc *= keep;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float w = __builtin_amdgcn_exp2f(ls[i] - use);
-      l += w;
-      acc += w * v[i];
-    }
-    m = mx;
+    merge_ranges(ls, v, m, l, acc);
   }
 #pragma unroll
   for (int o = 16; o < 64; o <<= 1) {
@@ -958,30 +974,50 @@ __device__ __forceinline__ void merge_row(const PagedArgs& p, int64_t first, int
     for (int j = 0; j < 4; ++j) acc[j] = acc[j] * wa + __shfl_xor(acc[j], o, 64) * wb;
     m = mx;
   }
-  if (g != 0) return;
-  const float inv = n > 0 ? 1.f / l : 0.f;
-  *reinterpret_cast<uint2*>(p.o + (int64_t)tok * p.orr + head * p.oh + d) =
-      uint2{pack16<F16>(acc[0] * inv, acc[1] * inv), pack16<F16>(acc[2] * inv, acc[3] * inv)};
-  if (p.lse && d == 0)
-    p.lse[(int64_t)head * p.new_rows + tok] = n > 0 ? ((m == -INFINITY ? 0.f : m) + __log2f(l)) * LN2 : -INFINITY;
+  if (g == 0) merge_store<F16>(p, n, m, l, acc, tok, head, d);
 }
 
-// The split tasks of the chunk kernel: blockIdx.x = task, blockIdx.y = 4 of its 128 rows
+// The split tasks of the chunk kernel: blockIdx.x = task, blockIdx.y = 32 of its 128 rows; 16 lanes x 4 columns per row
+// (there are many rows, so nothing is gained by spreading a row's ranges over lanes)
 template <bool F16>
 __global__ void __launch_bounds__(NT) attn_paged_merge_chunk(PagedArgs p) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int j = blockIdx.x, r = blockIdx.y * 4 + wave;
+  const int lane = threadIdx.x & 63, d = (threadIdx.x & 15) * 4;
+  const int j = blockIdx.x;
   int hk, tile;
   task_coords(p, p.whole + j, hk, tile);
   const RowTile rt = find_tile(p, tile, lane);
   if (rt.seq < 0) return;
   const int len = checked_len(p.kv_lens[rt.seq], p.cap, p.fault);
-  const int t0 = rt.tile * p.per_tile;
-  const int t = r / p.group;
-  if (t >= min(p.per_tile, rt.nq - t0)) return;
-  const int limit = key_limit(len - rt.nq + t0 + t, len, p.block);
-  merge_row<F16, QB>(p, (int64_t)j * p.splits * QB + r, (limit + p.chunk - 1) / p.chunk, rt.c0 + t0 + t,
-                     hk * p.group + r - t * p.group, lane);
+  const int t0 = rt.tile * p.per_tile, pos0 = len - rt.nq + t0;
+  const int rows = min(p.per_tile, rt.nq - t0) * p.group;
+  if (key_limit(pos0 + (rows - 1) / p.group, len, p.block) <= p.chunk) return;  // one range: written where computed
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = blockIdx.y * 32 + i * 16 + (threadIdx.x >> 4);
+    if (r >= rows) return;
+    const int t = r / p.group, tok = rt.c0 + t0 + t, head = hk * p.group + r - t * p.group;
+    const int n = (key_limit(pos0 + t, len, p.block) + p.chunk - 1) / p.chunk;
+    const int64_t first = (int64_t)j * p.splits * QB + r;
+    float m = -INFINITY, l = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int s0 = 0; s0 < n; s0 += 8) {
+      float ls[8];
+      f32x4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        ls[k] = -INFINITY;
+        v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (s0 + k < n) {
+          const int64_t at = first + (int64_t)(s0 + k) * QB;
+          ls[k] = p.part_lse[at];
+          v[k] = *reinterpret_cast<const f32x4*>(p.part_o + at * HD + d);
+        }
+      }
+      merge_ranges(ls, v, m, l, acc);
+    }
+    merge_store<F16>(p, n, m, l, acc, tok, head, d);
+  }
 }
 
 // The step kernel's rows: blockIdx.x = (sequence, K/V head), blockIdx.y = 4 of its rows
@@ -994,6 +1030,7 @@ __global__ void __launch_bounds__(NT) attn_paged_merge_step(PagedArgs p) {
   const int nq = new_tokens(p, c0, p.cu[b + 1]);
   if (r >= nq * p.group) return;
   const int len = checked_len(p.kv_lens[b], p.cap, p.fault);
+  if (key_limit(len - 1, len, p.block) <= p.chunk) return;  // one range: written where computed
   const int t = r / p.group;
   const int limit = key_limit(len - nq + t, len, p.block);
   merge_row<F16, RS>(p, (int64_t)blockIdx.x * p.splits * RS + r, (limit + p.chunk - 1) / p.chunk, c0 + t,
@@ -1121,7 +1158,7 @@ int launch_all(const PagedArgs& a, const Plan& pl, int page_dtype, int64_t wgs, 
   MAPA_CHECK_LAUNCH("mapa_attention_paged");
   if (pl.slots == 0) return 0;
   if (pl.rb == 0) {
-    const dim3 grid(a.tiles * a.kv_heads - a.whole, QB / 4);
+    const dim3 grid(a.tiles * a.kv_heads - a.whole, QB / 32);
     hipLaunchKernelGGL((attn_paged_merge_chunk<F16>), grid, dim3(NT), 0, stream, a);
   } else {
     const dim3 grid(a.seqs * a.kv_heads, (std::min(a.max_new * a.group, 16 * pl.rb) + 3) / 4);

@@ -26,24 +26,42 @@ struct CopyArgs {
   int64_t rs[2], hs[2];
   unsigned* fault;
   int seqs, table_stride, rows, cap, heads, psl, num_pages, tb;
+  uint32_t div_heads;  // small_div's multiplier of the head count
 };
 
-struct Place {
-  int seq, pos;
-};
+constexpr int U = 4;  // rows in flight per group of eight lanes
 
-// 8 values of a row in fp32
+// n / d for 0 <= n < 2^16 and 0 < d < 2^14 (m = ceil(2^31 / d))
+__device__ __forceinline__ int small_div(int n, uint32_t m) { return (int)__umulhi((uint32_t)n << 1, m); }
+
+// largest of the eight lanes of a row
+__device__ __forceinline__ uint32_t max8(uint32_t m) {
+  m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xf, 0xf, true));  // quad_perm 1, 0, 3, 2
+  m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xf, 0xf, true));  // quad_perm 2, 3, 0, 1
+  return max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x141, 0xf, 0xf, true));  // row_half_mirror: 7 - lane
+}
+
+// 8 values of a row as they lie in memory
+struct Float8 {
+  f32x4 a, b;
+};
 template <int DT>
-__device__ __forceinline__ void ld8(const void* p, float* f) {
+struct Row8 {
+  typedef uint4 T;
+};
+template <>
+struct Row8<MAPA_F32> {
+  typedef Float8 T;
+};
+template <int DT>
+__device__ __forceinline__ void unpack8(const typename Row8<DT>::T& u, float* f) {
   if constexpr (DT == MAPA_F32) {
-    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      f[j] = a[j];
-      f[4 + j] = b[j];
+      f[j] = u.a[j];
+      f[4 + j] = u.b[j];
     }
   } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -53,15 +71,12 @@ __device__ __forceinline__ void ld8(const void* p, float* f) {
   }
 }
 template <int DT>
-__device__ __forceinline__ void st8(void* p, const float* f) {
-  if constexpr (DT == MAPA_F32) {
-    reinterpret_cast<f32x4*>(p)[0] = f32x4{f[0], f[1], f[2], f[3]};
-    reinterpret_cast<f32x4*>(p)[1] = f32x4{f[4], f[5], f[6], f[7]};
-  } else {
-    *reinterpret_cast<uint4*>(p) =
-        uint4{pack_lp2(DT == MAPA_F16, f[0], f[1]), pack_lp2(DT == MAPA_F16, f[2], f[3]),
-              pack_lp2(DT == MAPA_F16, f[4], f[5]), pack_lp2(DT == MAPA_F16, f[6], f[7])};
-  }
+__device__ __forceinline__ typename Row8<DT>::T pack8(const float* f) {
+  if constexpr (DT == MAPA_F32)
+    return Float8{f32x4{f[0], f[1], f[2], f[3]}, f32x4{f[4], f[5], f[6], f[7]}};
+  else
+    return uint4{pack_lp2(DT == MAPA_F16, f[0], f[1]), pack_lp2(DT == MAPA_F16, f[2], f[3]),
+                 pack_lp2(DT == MAPA_F16, f[4], f[5]), pack_lp2(DT == MAPA_F16, f[6], f[7])};
 }
 
 // Sequence of each of the workgroup's rows t0 .. t0 + nt - 1 into `seq` (-1: none), by the packed offsets cu.
@@ -105,47 +120,66 @@ __global__ void __launch_bounds__(TPB) kv_write_kernel(CopyArgs a) {
   }
   __syncthreads();
 
+  // rows (token, K or V, head); the eight lanes of a row stay together, U rows per lane group in flight
   const int rows = nt * 2 * a.heads;
   const int l8 = threadIdx.x & 7;
-  for (int r = threadIdx.x >> 3; r < rows; r += TPB / 8) {  // the eight lanes of a row stay together
-    const int tk = r / a.heads, h = r - tk * a.heads, tl = tk >> 1, kv = tk & 1;
-    const int64_t to = at[tl];
-    if (to < 0) continue;
-    const int64_t dst = to + ((int64_t)h << a.psl);
-    const int64_t src = (int64_t)(t0 + tl) * a.rs[kv] + h * a.hs[kv] + l8 * 8;
-    if constexpr (SRC == PAGE) {
-      reinterpret_cast<uint4*>(a.page[kv])[dst * 8 + l8] =
-          *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.row[kv]) + src);
-    } else {
-      float f[8];
-      ld8<SRC>(reinterpret_cast<const char*>(a.row[kv]) + src * (SRC == MAPA_F32 ? 4 : 2), f);
-      if constexpr (!CODES) {
-        st8<PAGE>(reinterpret_cast<uint16_t*>(a.page[kv]) + dst * HD + l8 * 8, f);
+  for (int r0 = threadIdx.x >> 3; r0 < rows; r0 += U * (TPB / 8)) {
+    typename Row8<SRC>::T x[U];
+    int64_t dst[U];
+    bool isv[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const int r = r0 + k * (TPB / 8);
+      const int tk = small_div(r, a.div_heads), h = r - tk * a.heads, tl = tk >> 1;
+      isv[k] = tk & 1;
+      dst[k] = -1;
+      if (r < rows && at[tl] >= 0) {
+        dst[k] = at[tl] + ((int64_t)h << a.psl);
+        const int64_t src = (int64_t)(t0 + tl) * (isv[k] ? a.rs[1] : a.rs[0]) + h * (isv[k] ? a.hs[1] : a.hs[0]) + l8 * 8;
+        x[k] = *reinterpret_cast<const typename Row8<SRC>::T*>(
+            reinterpret_cast<const char*>(isv[k] ? a.row[1] : a.row[0]) + src * (SRC == MAPA_F32 ? 4 : 2));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (dst[k] < 0) continue;  // the same for the eight lanes of the row
+      void* page = isv[k] ? a.page[1] : a.page[0];
+      if constexpr (SRC == PAGE) {
+        reinterpret_cast<uint4*>(page)[dst[k] * 8 + l8] = __builtin_bit_cast(uint4, x[k]);
       } else {
-        uint32_t m = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(f[j]) & 0x7fffffffu);
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
-        const uint32_t e = row_exponent<PAGE == MAPA_I8>(m);
-        const float inv = exponent_inverse(e);
-        uint2 w;
-        if constexpr (PAGE == MAPA_FP8) {
-          int lo = 0, hi = 0;
-          lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0] * inv, f[1] * inv, lo, false);
-          lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[2] * inv, f[3] * inv, lo, true);
-          hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[4] * inv, f[5] * inv, hi, false);
-          hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[6] * inv, f[7] * inv, hi, true);
-          w = uint2{(uint32_t)lo, (uint32_t)hi};
-          if (e == 255u) w = uint2{0x7f7f7f7fu, 0x7f7f7f7fu};  // e4m3's NaN
+        float f[8];
+        unpack8<SRC>(x[k], f);
+        if constexpr (!CODES) {
+          reinterpret_cast<uint4*>(page)[dst[k] * 8 + l8] = __builtin_bit_cast(uint4, pack8<PAGE>(f));
         } else {
-          uint32_t c[8];
+          uint32_t m = 0;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) c[j] = (uint32_t)(int)rintf(e == 255u ? 0.f : f[j] * inv) & 0xffu;
-          w = uint2{c[0] | (c[1] << 8) | (c[2] << 16) | (c[3] << 24), c[4] | (c[5] << 8) | (c[6] << 16) | (c[7] << 24)};
+          for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(f[j]) & 0x7fffffffu);
+          m = max8(m);
+          const uint32_t e = row_exponent<PAGE == MAPA_I8>(m);
+          const float inv = exponent_inverse(e);
+          uint2 w;
+          if constexpr (PAGE == MAPA_FP8) {
+            int lo = 0, hi = 0;
+            lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[0] * inv, f[1] * inv, lo, false);
+            lo = __builtin_amdgcn_cvt_pk_fp8_f32(f[2] * inv, f[3] * inv, lo, true);
+            hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[4] * inv, f[5] * inv, hi, false);
+            hi = __builtin_amdgcn_cvt_pk_fp8_f32(f[6] * inv, f[7] * inv, hi, true);
+            w = uint2{(uint32_t)lo, (uint32_t)hi};
+            if (e == 255u) w = uint2{0x7f7f7f7fu, 0x7f7f7f7fu};  // e4m3's NaN
+          } else {
+            // x 2^-e + 1.5 2^23: the sum's last bits are the integer, rounded to nearest even (|code| <= 127)
+            uint32_t c[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) c[j] = __float_as_uint(__builtin_fmaf(f[j], inv, 12582912.f));
+            const uint32_t c01 = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), c23 = __builtin_amdgcn_perm(c[3], c[2], 0x04000c0cu);
+            const uint32_t c45 = __builtin_amdgcn_perm(c[5], c[4], 0x0c0c0400u), c67 = __builtin_amdgcn_perm(c[7], c[6], 0x04000c0cu);
+            w = uint2{c01 | c23, c45 | c67};
+            if (e == 255u) w = uint2{0u, 0u};
+          }
+          reinterpret_cast<uint2*>(page)[dst[k] * 8 + l8] = w;
+          if (l8 == 0) (isv[k] ? a.exp[1] : a.exp[0])[dst[k]] = (uint8_t)e;
         }
-        reinterpret_cast<uint2*>(a.page[kv])[dst * 8 + l8] = w;
-        if (l8 == 0) a.exp[kv][dst] = (uint8_t)e;
       }
     }
   }
@@ -175,32 +209,52 @@ __global__ void __launch_bounds__(TPB) kv_read_kernel(CopyArgs a) {
 
   const int rows = nt * 2 * a.heads;
   const int l8 = threadIdx.x & 7;
-  for (int r = threadIdx.x >> 3; r < rows; r += TPB / 8) {
-    const int tk = r / a.heads, h = r - tk * a.heads, tl = tk >> 1, kv = tk & 1;
-    const int64_t from = at[tl];
-    if (from == -2) continue;
-    const int64_t src = from + ((int64_t)h << a.psl);
-    char* dst = reinterpret_cast<char*>(a.row[kv]) +
-                ((int64_t)(t0 + tl) * a.rs[kv] + h * a.hs[kv] + l8 * 8) * (OUT == MAPA_F32 ? 4 : 2);
-    if constexpr (PAGE == OUT) {
-      *reinterpret_cast<uint4*>(dst) = from < 0 ? uint4{0, 0, 0, 0} : reinterpret_cast<const uint4*>(a.page[kv])[src * 8 + l8];
-    } else {
-      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (from >= 0) {
-        if constexpr (!CODES) {
-          ld8<PAGE>(reinterpret_cast<const uint16_t*>(a.page[kv]) + src * HD + l8 * 8, f);
-        } else {
-          const uint2 w = reinterpret_cast<const uint2*>(a.page[kv])[src * 8 + l8];
-          const float s = exponent_value(a.exp[kv][src]);
-          const f32x4 x = decode4<PAGE == MAPA_I8>(w.x, s), y = decode4<PAGE == MAPA_I8>(w.y, s);
+  for (int r0 = threadIdx.x >> 3; r0 < rows; r0 += U * (TPB / 8)) {
+    uint4 x[U];  // 16-bit pages: 8 values; codes: 8 codes and the exponent byte
+    char* dst[U];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            f[j] = x[j];
-            f[4 + j] = y[j];
+    for (int k = 0; k < U; ++k) {
+      const int r = r0 + k * (TPB / 8);
+      const int tk = small_div(r, a.div_heads), h = r - tk * a.heads, tl = tk >> 1;
+      const bool isv = tk & 1;
+      dst[k] = nullptr;
+      x[k] = uint4{0, 0, 0, 0};
+      if (r < rows && at[tl] != -2) {
+        const int64_t from = at[tl], src = from + ((int64_t)h << a.psl);
+        dst[k] = reinterpret_cast<char*>(isv ? a.row[1] : a.row[0]) +
+                 ((int64_t)(t0 + tl) * (isv ? a.rs[1] : a.rs[0]) + h * (isv ? a.hs[1] : a.hs[0]) + l8 * 8) *
+                     (OUT == MAPA_F32 ? 4 : 2);
+        if (from >= 0) {
+          const void* page = isv ? a.page[1] : a.page[0];
+          if constexpr (!CODES) {
+            x[k] = reinterpret_cast<const uint4*>(page)[src * 8 + l8];
+          } else {
+            const uint2 w = reinterpret_cast<const uint2*>(page)[src * 8 + l8];
+            x[k] = uint4{w.x, w.y, (isv ? a.exp[1] : a.exp[0])[src], 0};
           }
         }
       }
-      st8<OUT>(dst, f);
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (!dst[k]) continue;
+      if constexpr (PAGE == OUT) {
+        *reinterpret_cast<uint4*>(dst[k]) = x[k];
+      } else {
+        float f[8];
+        if constexpr (!CODES) {
+          unpack8<PAGE>(x[k], f);
+        } else {
+          const float s = exponent_value(x[k].z);
+          const f32x4 lo = decode4<PAGE == MAPA_I8>(x[k].x, s), hi = decode4<PAGE == MAPA_I8>(x[k].y, s);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            f[j] = lo[j];
+            f[4 + j] = hi[j];
+          }
+        }
+        *reinterpret_cast<typename Row8<OUT>::T*>(dst[k]) = pack8<OUT>(f);
+      }
     }
   }
 }
@@ -244,6 +298,7 @@ int fill_args(CopyArgs& a, const mapa_kv_cache* c, const mapa_kv_batch* b, const
   a.fault = mapa_gemm_impl::fault_word();
   a.seqs = b->seqs; a.table_stride = b->table_stride;
   a.cap = kv_cap(*c, *b);
+  a.div_heads = ((1u << 31) + c->heads - 1) / c->heads;
   a.heads = c->heads; a.psl = log2_of(c->page_size); a.num_pages = c->num_pages;
   return 0;
 }

@@ -66,7 +66,7 @@ __device__ __forceinline__ f32x4 decode4(uint32_t w, float s) {
 inline int check_cache(const mapa_kv_cache& c, const char* who) {
   MAPA_CHECK_ARG(c.dtype == MAPA_BF16 || c.dtype == MAPA_F16 || c.dtype == MAPA_FP8 || c.dtype == MAPA_I8,
                  "%s: pages must be bf16, f16, fp8 or i8", who);
-  MAPA_CHECK_ARG(c.heads > 0 && c.heads <= 65535 && c.num_pages > 0, "%s: bad cache (%d heads, %d pages)", who, c.heads,
+  MAPA_CHECK_ARG(c.heads > 0 && c.heads <= 2048 && c.num_pages > 0, "%s: bad cache (%d heads, %d pages)", who, c.heads,
                  c.num_pages);
   MAPA_CHECK_ARG(c.page_size >= 16 && c.page_size <= 1024 && (c.page_size & (c.page_size - 1)) == 0,
                  "%s: page size %d must be a power of two, 16 to 1024", who, c.page_size);

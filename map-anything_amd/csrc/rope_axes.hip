@@ -4,7 +4,8 @@
 // Memory-bound: every value is read and written once, 3 flop per value, and a token's S cosines and sines serve all of
 // its heads (both tensors).  A workgroup takes TB tokens: one thread per (token, pair) computes its cosine and sine
 // into LDS, then the threads walk the tokens' (head, group of W pairs) items in the tensor's own memory order, 16 B per
-// access where sections and strides allow.  The angle is formed and reduced to a fraction of a turn in 64 bits (a
+// access where sections and strides allow.  A thread keeps its group of pairs for all of its items, so an item costs
+// one small division and two LDS address lookups beside its loads.  The angle is formed and reduced to a fraction of a turn in 64 bits (a
 // far time times a frequency of one keeps no fraction in 32), then sincospif; per token that is S of them against
 // 2 * heads * S values moved.
 #include "mapa_common.h"
@@ -22,6 +23,8 @@ struct RopeArgs {
   const void* pos;
   int64_t pb, pn, pa;
   int pos_f32, batch, tokens, S, rest, tb, head_major;
+  int den;       // items of the inner loop: tb tokens or all heads
+  uint32_t div;  // small_div's multiplier of den
   int first[MAPA_ROPE_MAX_AXES + 1];  // first pair of each axis (unused axes: S)
   float sign;
   double turns[MAPA_ROPE_MAX_PAIRS];  // turns per unit of position
@@ -75,11 +78,15 @@ __device__ __forceinline__ void st(typename Elem<DT>::T* p, const Vec<DT, N>& v)
   *reinterpret_cast<W*>(p) = __builtin_bit_cast(W, v);
 }
 
+// n / d for 0 <= n < 2^16, 0 < d < 2^14 (m = ceil(2^31 / d))
+__device__ __forceinline__ int small_div(int n, uint32_t m) { return (int)__umulhi((uint32_t)n << 1, m); }
+
 // W pairs per item; PAIRED: u and v are neighbours (interleaved columns), one access of 2 W values instead of two of W
 template <int DT, int W, bool PAIRED, bool AXIAL>
 __global__ void __launch_bounds__(TPB) rope_axes_kernel(RopeArgs a) {
   typedef typename Elem<DT>::T T;
   __shared__ __attribute__((aligned(16))) float cs[MAX_TB * MAPA_ROPE_MAX_PAIRS], sn[MAX_TB * MAPA_ROPE_MAX_PAIRS];
+  __shared__ int64_t xat[2][MAX_TB], yat[2][MAX_TB];  // element offsets of the workgroup's tokens
   const int total = a.batch * a.tokens;  // fits (checked on the host)
   const int t0 = blockIdx.x * a.tb;
   const int nt = min(total - t0, a.tb);
@@ -90,6 +97,13 @@ __global__ void __launch_bounds__(TPB) rope_axes_kernel(RopeArgs a) {
     const int64_t at = b * a.pb + n * a.pn + ax * a.pa;
     const double p = a.pos_f32 ? (double)reinterpret_cast<const float*>(a.pos)[at]
                                : (double)reinterpret_cast<const int64_t*>(a.pos)[at];
+    if (i == 0) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        xat[w][tl] = b * a.xb[w] + n * a.xn[w];
+        yat[w][tl] = b * a.yb[w] + n * a.yn[w];
+      }
+    }
     const double turn = p * a.turns[i];
     float s, c;
     sincospif(2.f * (float)(turn - rint(turn)), &s, &c);
@@ -98,45 +112,40 @@ __global__ void __launch_bounds__(TPB) rope_axes_kernel(RopeArgs a) {
   }
   __syncthreads();
 
-  const int heads = a.heads[0] + a.heads[1], groups = a.S / W;
-  const int items = nt * heads * groups;
-  // item -> (token, head, group), walked as the tensor lies in memory: heads inside tokens, or tokens inside heads
-  auto split = [&](int it, int per, int& tl, int& h, int& g) __attribute__((always_inline)) {
-    const int q = it / per;
-    g = it - q * per;
-    if (a.head_major) {
-      h = q / nt;
-      tl = q - h * nt;
-    } else {
-      tl = q / heads;
-      h = q - tl * heads;
-    }
+  // items (token, head) of this thread's group of pairs, walked as the tensor lies in memory: heads inside tokens, or
+  // tokens inside heads
+  const int heads = a.heads[0] + a.heads[1], groups = a.S / W, rows = TPB / groups;
+  const int q0 = threadIdx.x / groups, i = (threadIdx.x - q0 * groups) * W;
+  int col = PAIRED ? 2 * i : i, step = a.S;
+  if constexpr (AXIAL) {  // the axis' block begins at column 2 first: u at i - first in it, v section columns on
+    const int f = i >= a.first[3] ? a.first[3] : i >= a.first[2] ? a.first[2] : i >= a.first[1] ? a.first[1] : 0;
+    const int e = i >= a.first[3] ? a.first[4] : i >= a.first[2] ? a.first[3] : i >= a.first[1] ? a.first[2] : a.first[1];
+    col = f + i;
+    step = e - f;
+  }
+  auto split = [&](int q, int& tl, int& h) __attribute__((always_inline)) {
+    const int outer = small_div(q, a.div), inner = q - outer * a.den;
+    tl = a.head_major ? inner : outer;
+    h = a.head_major ? outer : inner;
   };
+  // (a partial last workgroup walks the places of its missing tokens too, and skips them)
+  const int items = a.tb * heads;
   constexpr int U = 4;  // items in flight per thread
-  for (int base = threadIdx.x; base < items; base += TPB * U) {
+  for (int base = q0; base < items && q0 < rows; base += rows * U) {
     Vec<DT, PAIRED ? 2 * W : W> lo[U], hi[U];
     T* out[U];
-    int tab[U], step[U];
+    int tab[U];
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      const int it = base + k * TPB;
+      const int q = base + k * rows;
       out[k] = nullptr;
-      if (it < items) {
-        int tl, h, g;
-        split(it, groups, tl, h, g);
-        const int w = h >= a.heads[0];
+      int tl, h;
+      split(q, tl, h);
+      if (q < items && tl < nt) {
+        const bool w = h >= a.heads[0];
         const int hh = w ? h - a.heads[0] : h;
-        const int t = t0 + tl, b = t / a.tokens, n = t - b * a.tokens;
-        const int i = g * W;
-        int col = PAIRED ? 2 * i : i;
-        step[k] = a.S;
-        if constexpr (AXIAL) {
-          const int ax = (i >= a.first[1]) + (i >= a.first[2]) + (i >= a.first[3]);
-          step[k] = a.first[ax + 1] - a.first[ax];
-          col = a.first[ax] + i;  // 2 first + (i - first)
-        }
-        const T* src = reinterpret_cast<const T*>(a.x[w]) + b * a.xb[w] + hh * a.xh[w] + n * a.xn[w] + col;
-        out[k] = reinterpret_cast<T*>(a.y[w]) + b * a.yb[w] + hh * a.yh[w] + n * a.yn[w] + col;
+        const T* src = reinterpret_cast<const T*>(w ? a.x[1] : a.x[0]) + xat[w][tl] + hh * (w ? a.xh[1] : a.xh[0]) + col;
+        out[k] = reinterpret_cast<T*>(w ? a.y[1] : a.y[0]) + yat[w][tl] + hh * (w ? a.yh[1] : a.yh[0]) + col;
         tab[k] = tl * a.S + i;
         if constexpr (PAIRED && W == 1) {  // no alignment beyond the element's
           lo[k].e[0] = src[0];
@@ -145,7 +154,7 @@ __global__ void __launch_bounds__(TPB) rope_axes_kernel(RopeArgs a) {
           lo[k] = ld<DT, 2 * W>(src);
         } else {
           lo[k] = ld<DT, W>(src);
-          hi[k] = ld<DT, W>(src + step[k]);
+          hi[k] = ld<DT, W>(src + step);
         }
       }
     }
@@ -168,20 +177,21 @@ __global__ void __launch_bounds__(TPB) rope_axes_kernel(RopeArgs a) {
           st<DT, 2 * W>(out[k], lo[k]);
         } else {
           st<DT, W>(out[k], lo[k]);
-          st<DT, W>(out[k] + step[k], hi[k]);
+          st<DT, W>(out[k] + step, hi[k]);
         }
       }
     }
   }
   // the dims behind the rotated ones, copied (rest is 0 when the tensors are rotated in place)
-  for (int it = threadIdx.x; it < nt * heads * a.rest; it += TPB) {
-    int tl, h, c;
-    split(it, a.rest, tl, h, c);
-    const int w = h >= a.heads[0];
+  for (int it = threadIdx.x; it < items * a.rest; it += TPB) {
+    const int q = it / a.rest, c = it - q * a.rest;
+    int tl, h;
+    split(q, tl, h);
+    if (tl >= nt) continue;
+    const bool w = h >= a.heads[0];
     const int hh = w ? h - a.heads[0] : h;
-    const int t = t0 + tl, b = t / a.tokens, n = t - b * a.tokens;
-    reinterpret_cast<T*>(a.y[w])[b * a.yb[w] + hh * a.yh[w] + n * a.yn[w] + 2 * a.S + c] =
-        reinterpret_cast<const T*>(a.x[w])[b * a.xb[w] + hh * a.xh[w] + n * a.xn[w] + 2 * a.S + c];
+    reinterpret_cast<T*>(w ? a.y[1] : a.y[0])[yat[w][tl] + hh * (w ? a.yh[1] : a.yh[0]) + 2 * a.S + c] =
+        reinterpret_cast<const T*>(w ? a.x[1] : a.x[0])[xat[w][tl] + hh * (w ? a.xh[1] : a.xh[0]) + 2 * a.S + c];
   }
 }
 
@@ -239,7 +249,8 @@ extern "C" int mapa_rope_axes(const mapa_rope_axes_desc* d, hipStream_t stream) 
   bool in_place = true;
   int heads = 0;
   for (int i = 0; i < 2; ++i) {
-    MAPA_CHECK_ARG(d->heads[i] >= 0 && d->heads[i] <= 65536, "mapa_rope_axes: bad head count %d", d->heads[i]);
+    MAPA_CHECK_ARG(d->heads[i] >= 0 && d->heads[i] <= 2048, "mapa_rope_axes: bad head count %d (at most 2048)",
+                   d->heads[i]);
     a.heads[i] = d->x[i] ? d->heads[i] : 0;
     heads += a.heads[i];
     if (!a.heads[i]) continue;
@@ -287,6 +298,8 @@ extern "C" int mapa_rope_axes(const mapa_rope_axes_desc* d, hipStream_t stream) 
   a.head_major = a.xh[w0] > a.xn[w0];
   a.tb = 1;  // tokens per workgroup: one while that leaves fewer than four workgroups per CU
   while (a.tb < MAX_TB && total / (2 * a.tb) >= 1024) a.tb *= 2;
+  a.den = a.head_major ? a.tb : heads;
+  a.div = ((1u << 31) + a.den - 1) / a.den;
   const unsigned grid = (unsigned)((total + a.tb - 1) / a.tb);
   if (d->dtype == MAPA_F32) launch<MAPA_F32>(a, d->layout, W, grid, stream);
   else if (d->dtype == MAPA_BF16) launch<MAPA_BF16>(a, d->layout, W, grid, stream);

@@ -147,7 +147,7 @@ class PagedKVCache:
             raise nat.NativeError(f"PagedKVCache: cu_rows {tuple(cu_rows.shape)} does not fit the batch")
         heads = self.k.shape[1]
         if out is None:
-            out = tuple(torch.empty(rows, heads, HEAD_DIM, dtype=dtype, device=self.k.device) for _ in range(2))
+            out = tuple(batch.table.new_empty(rows, heads, HEAD_DIM, dtype=dtype) for _ in range(2))
         k, v = out
         for t, name in ((k, "k"), (v, "v")):
             self._rows(t, name, heads)
@@ -169,12 +169,12 @@ class PagedKVCache:
         self._rows(q, "q")
         self._same(batch)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            out = q.new_empty(q.shape)
         else:
             self._rows(out, "out", q.shape[1])
             if out.shape[0] != q.shape[0] or out.dtype != q.dtype:
                 raise nat.NativeError("PagedKVCache: out must have q's shape and dtype")
-        lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device) if return_lse else None
+        lse = q.new_empty(q.shape[1], q.shape[0], dtype=torch.float32) if return_lse else None
         with nat.on_device(self.k.device):
             nat.attention_paged(self.desc, batch._rows(q.shape[0]), q, out, lse=lse, scale=scale, mask_block=mask_block)
         return (out, lse) if return_lse else out

@@ -7,6 +7,8 @@ raises (mapanything._native).
     q = rope(q, positions)     # q (B, heads, N, D) bf16/fp32 on the GPU, positions (B, N, 2) int64 (y, x)
 """
 
+import struct
+
 import torch
 
 from mapanything import _native as nat
@@ -57,7 +59,10 @@ class _RoPEAxesTurn(torch.autograd.Function):
         first, second = (g_tokens, g_keys) if g_tokens is not None else (g_keys, None)
         if first is None:
             return (None,) * 5
-        a, b = _RoPEAxesTurn.apply(ctx.rope, not ctx.inverse, positions, first, second)
+        if torch.is_grad_enabled():  # a second derivative is asked for
+            a, b = _RoPEAxesTurn.apply(ctx.rope, not ctx.inverse, positions, first, second)
+        else:
+            a, b = ctx.rope._turn(first, second, positions, not ctx.inverse)
         return (None, None, None) + ((a, b) if g_tokens is not None else (None, a))
 
 
@@ -158,20 +163,26 @@ class RoPEAxes:
     def _run(self, a, b, positions, inverse, ya, yb):
         if not a.is_cuda:
             raise nat.NativeError("RoPEAxes: tensors must be on the GPU; there is no CPU path")
-        B, _, N, D = a.shape
+        B, H, N, D = a.shape
+        sa, ta, sp = a.stride(), ya.stride(), positions.stride()
+        if b is None:
+            second, sb, tb = (0, 0, 0), (0, 0, 0), (0, 0, 0)
+        else:
+            second, sb, tb = (b.data_ptr(), yb.data_ptr(), b.shape[1]), b.stride(), yb.stride()
         d = nat.RopeAxesDesc.from_buffer_copy(self._desc)
-        d.dtype, d.batch, d.tokens, d.head_dim, d.inverse = nat.dt_code(a.dtype), B, N, D, int(inverse)
-        for i, (x, y) in enumerate(((a, ya), (b, yb))):
-            if x is not None:
-                d.x[i], d.y[i], d.heads[i] = x.data_ptr(), y.data_ptr(), x.shape[1]
-                d.x_bstride[i], d.x_hstride[i], d.x_nstride[i], _ = x.stride()
-                d.y_bstride[i], d.y_hstride[i], d.y_nstride[i], _ = y.stride()
-        d.positions = positions.data_ptr()
-        d.pos_dtype = nat.POS_F32 if positions.dtype == torch.float32 else nat.POS_I64
-        pb, d.pos_nstride, d.pos_astride = positions.stride()
-        d.pos_bstride = pb if positions.shape[0] > 1 else 0
+        # the fields from dtype to pos_astride in one packing (setting them one by one costs more than the launch)
+        _DESC_HEAD.pack_into(d, 0, nat.dt_code(a.dtype), B, N, D, a.data_ptr(), second[0], ya.data_ptr(), second[1], H,
+                             second[2], sa[0], sb[0], sa[1], sb[1], sa[2], sb[2], ta[0], tb[0], ta[1], tb[1], ta[2],
+                             tb[2], positions.data_ptr(),
+                             nat.POS_F32 if positions.dtype == torch.float32 else nat.POS_I64,
+                             sp[0] if positions.shape[0] > 1 else 0, sp[1], sp[2])
+        d.inverse = int(inverse)
         with nat.on_device(a.device):
             nat.rope_axes(d)
+
+
+# include/mapa.h mapa_rope_axes_desc up to pos_astride: 4 ints, x, y, heads, 12 strides, positions, pos_dtype, 3 strides
+_DESC_HEAD = struct.Struct("=4i4Q2i12qQi4x3q")
 
 
 def _like(x):

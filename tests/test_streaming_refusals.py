@@ -44,7 +44,7 @@ def _rope(nat, **over):
     ({"pos_dtype": 2}, b"pos_dtype"), ({"section": (8, 0, 12)}, b"section"), ({"section": (8, 12, 13)}, b"do not fit"),
     ({"section": (120, 9, 1), "head_dim": 512}, b"do not fit"), ({"head_dim": 0}, b"bad shape"),
     ({"tokens": -1}, b"bad shape"), ({"y": (None, None)}, b"null output"), ({"positions": None}, b"null positions"),
-    ({"y_nstride": (64, 0)}, b"in place"), ({"x": (4097, None)}, b"aligned"), ({"heads": (-1, 0)}, b"head count"),
+    ({"y_nstride": (64, 0)}, b"in place"), ({"x": (4097, None)}, b"aligned"), ({"heads": (-1, 0)}, b"head count"), ({"heads": (2049, 0)}, b"head count"),
     ({"batch": 65536, "tokens": 65536}, b"too many"),
 ])
 def test_rope_axes_refuses(nat, over, word):
@@ -84,7 +84,7 @@ def _batch(nat, **over):
     return b
 
 
-CACHE_REFUSALS = [({"dtype": 0}, b"pages must be"), ({"heads": 0}, b"bad cache"), ({"num_pages": 0}, b"bad cache"),
+CACHE_REFUSALS = [({"dtype": 0}, b"pages must be"), ({"heads": 0}, b"bad cache"), ({"heads": 2049}, b"bad cache"), ({"num_pages": 0}, b"bad cache"),
                   ({"page_size": 8}, b"page size"), ({"page_size": 48}, b"page size"),
                   ({"page_size": 2048}, b"page size"), ({"k": None}, b"aligned"), ({"v": 8200}, b"aligned"),
                   ({"dtype": 5}, b"exponent"), ({"dtype": 6, "k_exp": 64}, b"exponent")]
@@ -181,3 +181,11 @@ def test_descriptor_layouts_match_header(tmp_path, nat):
         assert got[(cname, "sizeof")] == ctypes.sizeof(cls), cname
         for f, _ in cls._fields_:
             assert got[(cname, f)] == getattr(cls, f).offset, (cname, f)
+    from uniception.models.libs.croco import pos_embed
+
+    assert pos_embed._DESC_HEAD.size == nat.RopeAxesDesc.axes.offset  # what RoPEAxes packs at once
+    d = nat.RopeAxesDesc()
+    pos_embed._DESC_HEAD.pack_into(d, 0, *range(1, 28))
+    flat = [d.dtype, d.batch, d.tokens, d.head_dim, *d.x, *d.y, *d.heads, *d.x_bstride, *d.x_hstride, *d.x_nstride,
+            *d.y_bstride, *d.y_hstride, *d.y_nstride, d.positions, d.pos_dtype, d.pos_bstride, d.pos_nstride, d.pos_astride]
+    assert flat == list(range(1, 28))
