@@ -4,8 +4,9 @@
 // values: eight lanes hold a row, eight values each (16 B of a 16-bit row), so its largest value is three exchanges
 // away and a wave moves eight whole rows.  A workgroup takes a few tokens; its threads find their sequences by looking
 // at all row offsets at once (thread i holds the interval of sequence i: one trip to memory however many sequences
-// there are, where a binary search makes log2 of them), one thread per token looks its page up, and the (token, K or V,
-// head) rows follow in an order that keeps neighbouring lanes on neighbouring memory.
+// there are, where a binary search makes log2 of them) and one thread per token looks its page up.  The rows follow as
+// (K or V, head, token): a wave's eight rows are neighbours in the page (512 B of 8-bit codes and eight exponent bytes
+// in a row), where (token, head) order scatters them over eight heads' parts of it.
 #include <type_traits>
 
 #include "paged.h"
@@ -25,14 +26,11 @@ struct CopyArgs {
   void* row[2];
   int64_t rs[2], hs[2];
   unsigned* fault;
-  int seqs, table_stride, rows, cap, heads, psl, num_pages, tb;
-  uint32_t div_heads;  // small_div's multiplier of the head count
+  int seqs, table_stride, rows, cap, heads, psl, num_pages;
+  int tb, tbl;  // tokens per workgroup (a power of two), its logarithm
 };
 
 constexpr int U = 4;  // rows in flight per group of eight lanes
-
-// n / d for 0 <= n < 2^16 and 0 < d < 2^14 (m = ceil(2^31 / d))
-__device__ __forceinline__ int small_div(int n, uint32_t m) { return (int)__umulhi((uint32_t)n << 1, m); }
 
 // largest of the eight lanes of a row
 __device__ __forceinline__ uint32_t max8(uint32_t m) {
@@ -102,8 +100,8 @@ __global__ void __launch_bounds__(TPB) kv_write_kernel(CopyArgs a) {
   __shared__ int64_t at[MAX_TB];  // row of the page that takes the token, for head 0; -1: nothing to write
   const int t0 = blockIdx.x * a.tb, nt = min(a.rows - t0, a.tb);
   find_sequences(a, t0, nt, seq);
-  if (threadIdx.x < nt) {
-    const int t = t0 + threadIdx.x, b = seq[threadIdx.x];
+  if (threadIdx.x < a.tb) {
+    const int t = t0 + threadIdx.x, b = seq[threadIdx.x];  // -1 past the last row
     int64_t r = -1;
     if (b >= 0) {
       const int c0 = a.cu[b], c1 = a.cu[b + 1];
@@ -120,8 +118,8 @@ __global__ void __launch_bounds__(TPB) kv_write_kernel(CopyArgs a) {
   }
   __syncthreads();
 
-  // rows (token, K or V, head); the eight lanes of a row stay together, U rows per lane group in flight
-  const int rows = nt * 2 * a.heads;
+  // rows (K or V, head, token); the eight lanes of a row stay together, U rows per lane group in flight
+  const int rows = 2 * a.heads << a.tbl;
   const int l8 = threadIdx.x & 7;
   for (int r0 = threadIdx.x >> 3; r0 < rows; r0 += U * (TPB / 8)) {
     typename Row8<SRC>::T x[U];
@@ -130,8 +128,9 @@ __global__ void __launch_bounds__(TPB) kv_write_kernel(CopyArgs a) {
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int r = r0 + k * (TPB / 8);
-      const int tk = small_div(r, a.div_heads), h = r - tk * a.heads, tl = tk >> 1;
-      isv[k] = tk & 1;
+      const int kh = r >> a.tbl, tl = r & (a.tb - 1);
+      isv[k] = kh >= a.heads;
+      const int h = isv[k] ? kh - a.heads : kh;
       dst[k] = -1;
       if (r < rows && at[tl] >= 0) {
         dst[k] = at[tl] + ((int64_t)h << a.psl);
@@ -192,8 +191,8 @@ __global__ void __launch_bounds__(TPB) kv_read_kernel(CopyArgs a) {
   __shared__ int64_t at[MAX_TB];  // row of the page that holds the token, for head 0; -1: zero, -2: not a row of ours
   const int t0 = blockIdx.x * a.tb, nt = min(a.rows - t0, a.tb);
   find_sequences(a, t0, nt, seq);
-  if (threadIdx.x < nt) {
-    const int b = seq[threadIdx.x];
+  if (threadIdx.x < a.tb) {
+    const int b = seq[threadIdx.x];  // -1 past the last row
     int64_t r = -2;
     if (b >= 0) {
       const int pos = t0 + threadIdx.x - a.cu[b];
@@ -207,7 +206,7 @@ __global__ void __launch_bounds__(TPB) kv_read_kernel(CopyArgs a) {
   }
   __syncthreads();
 
-  const int rows = nt * 2 * a.heads;
+  const int rows = 2 * a.heads << a.tbl;
   const int l8 = threadIdx.x & 7;
   for (int r0 = threadIdx.x >> 3; r0 < rows; r0 += U * (TPB / 8)) {
     uint4 x[U];  // 16-bit pages: 8 values; codes: 8 codes and the exponent byte
@@ -215,8 +214,9 @@ __global__ void __launch_bounds__(TPB) kv_read_kernel(CopyArgs a) {
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const int r = r0 + k * (TPB / 8);
-      const int tk = small_div(r, a.div_heads), h = r - tk * a.heads, tl = tk >> 1;
-      const bool isv = tk & 1;
+      const int kh = r >> a.tbl, tl = r & (a.tb - 1);
+      const bool isv = kh >= a.heads;
+      const int h = isv ? kh - a.heads : kh;
       dst[k] = nullptr;
       x[k] = uint4{0, 0, 0, 0};
       if (r < rows && at[tl] != -2) {
@@ -298,7 +298,6 @@ int fill_args(CopyArgs& a, const mapa_kv_cache* c, const mapa_kv_batch* b, const
   a.fault = mapa_gemm_impl::fault_word();
   a.seqs = b->seqs; a.table_stride = b->table_stride;
   a.cap = kv_cap(*c, *b);
-  a.div_heads = ((1u << 31) + c->heads - 1) / c->heads;
   a.heads = c->heads; a.psl = log2_of(c->page_size); a.num_pages = c->num_pages;
   return 0;
 }
@@ -324,6 +323,7 @@ extern "C" int mapa_kv_cache_write(const mapa_kv_cache* c, const mapa_kv_batch* 
   a.cu = b->cu_new;
   a.rows = b->new_rows;
   a.tb = tokens_per_block(a.rows);
+  a.tbl = log2_of(a.tb);
   const dim3 grid((unsigned)((a.rows + a.tb - 1) / a.tb));
   by_row(dtype, [&](auto src) {
     by_page(c->dtype, [&](auto page) {
@@ -350,6 +350,7 @@ extern "C" int mapa_kv_cache_read(const mapa_kv_cache* c, const mapa_kv_batch* b
   a.cu = cu_rows;
   a.rows = rows;
   a.tb = tokens_per_block(a.rows);
+  a.tbl = log2_of(a.tb);
   const dim3 grid((unsigned)((a.rows + a.tb - 1) / a.tb));
   by_row(dtype, [&](auto out) {
     by_page(c->dtype, [&](auto page) {

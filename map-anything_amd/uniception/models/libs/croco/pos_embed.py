@@ -99,7 +99,7 @@ class RoPEAxes:
             raise ValueError(f"RoPEAxes: freq must be positive, got {freq}")
         self.sections, self.base, self.F0 = sections, float(freq), float(F0)
         self.layout, self.spectrum = layout, spectrum
-        pairs = sum(sections)
+        self._pairs = pairs = sum(sections)
         if spectrum == "axis":
             part = [j / n for n in sections for j in range(n)]
         else:
@@ -115,21 +115,17 @@ class RoPEAxes:
         return self.forward(tokens, positions, keys, inplace)
 
     def forward(self, tokens, positions, keys=None, inplace: bool = False):
-        for name, t in (("tokens", tokens), ("keys", keys)):
-            if t is None:
-                continue
-            if t.ndim != 4 or 2 * sum(self.sections) > t.shape[3]:
-                raise ValueError(f"RoPEAxes: {name} {tuple(t.shape)} must be (B, H, N, D) with D >= "
-                                 f"{2 * sum(self.sections)}")
-            if t.device != tokens.device or t.dtype != tokens.dtype or t.shape[2:] != tokens.shape[2:] or \
-                    t.shape[0] != tokens.shape[0]:
+        self._check(tokens, "tokens")
+        B, _, N, D = tokens.shape
+        if keys is not None:
+            self._check(keys, "keys")
+            b, _, n, d = keys.shape
+            if b != B or n != N or d != D or keys.dtype != tokens.dtype or keys.device != tokens.device:
                 raise ValueError("RoPEAxes: tokens and keys must share device, dtype, batch, length and head dim")
-            if t.stride(3) != 1 and t.shape[3] > 1:
-                raise ValueError("RoPEAxes: the head dimension must be contiguous")
-        B, _, N, _ = tokens.shape
         if positions.ndim == 2:
             positions = positions[None]
-        if positions.ndim != 3 or positions.shape[0] not in (1, B) or positions.shape[1:] != (N, len(self.sections)):
+        if positions.ndim != 3 or positions.shape[0] not in (1, B) or positions.shape[1] != N or \
+                positions.shape[2] != len(self.sections):
             raise ValueError(f"RoPEAxes: positions {tuple(positions.shape)} do not match tokens (B={B}, N={N}) and "
                              f"{len(self.sections)} axes")
         if positions.dtype != torch.int64 and positions.dtype != torch.float32:
@@ -152,6 +148,12 @@ class RoPEAxes:
         else:
             out = self._turn(tokens, keys, positions, False)
         return out[0] if keys is None else out
+
+    def _check(self, t, name):
+        if t.ndim != 4 or 2 * self._pairs > t.shape[3]:
+            raise ValueError(f"RoPEAxes: {name} {tuple(t.shape)} must be (B, H, N, D) with D >= {2 * self._pairs}")
+        if t.stride(3) != 1 and t.shape[3] > 1:
+            raise ValueError("RoPEAxes: the head dimension must be contiguous")
 
     def _turn(self, tokens, keys, positions, inverse):
         a = tokens if tokens.stride(3) == 1 else tokens.contiguous()  # a gradient may come expanded
@@ -189,5 +191,5 @@ def _like(x):
     """An empty (B, H, N, D) tensor laid out as x is: heads inside tokens, or tokens inside heads."""
     B, H, N, D = x.shape
     if x.stride(1) < x.stride(2):
-        return x.new_empty(B, N, H, D).transpose(1, 2)
-    return x.new_empty(B, H, N, D)
+        return x.new_empty_strided((B, H, N, D), (N * H * D, D, H * D, 1))
+    return x.new_empty((B, H, N, D))
