@@ -94,11 +94,7 @@ __device__ __forceinline__ int new_tokens(const PagedArgs& p, int c0, int c1) {
   return c1 - c0;
 }
 
-// The wave's view of a sequence's page table: lane i holds the (checked) page of logical page w0 + i, so a page number
-// is a v_readlane away from being a scalar; a new window is fetched every 64 pages.
-struct PageWindow {
-  int w0, pages;
-};
+// Page w0 + lane of a sequence with `pages` of them, held within the cache.
 __device__ __forceinline__ int load_window(const PagedArgs& p, const int32_t* row, int w0, int pages, int lane) {
   int v = 0;
   if (w0 + lane < pages) v = checked_page(row[w0 + lane], p.num_pages, p.fault);
@@ -648,6 +644,62 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
 
   // (sequence, key range, K/V head): the heads of a range innermost, so that one table row serves neighbours
   const int hk = blockIdx.x % p.kv_heads, bs = blockIdx.x / p.kv_heads, split = bs % p.splits, b = bs / p.splits;
+  // The page window and, for one sequence alone, the first tiles are fetched before its length is known (the range's
+  // place is not a matter of it; what lies past the sequence is hidden later): one trip to memory less in a chain of
+  // four.  Of several sequences most ranges may be past the end, and other workgroups cover the wait.  Pages are held
+  // within the cache here and reported once the length says which of them are the sequence's.
+  const int32_t* trow = p.table + (int64_t)b * p.table_stride;
+  const int k_begin = split * p.chunk;
+  const int pmask = (1 << p.psl) - 1;
+  const int64_t page_rows = (int64_t)p.kv_heads << p.psl, head_rows = (int64_t)hk << p.psl;
+  int w0 = k_begin >> p.psl, raw = 0;
+  int64_t win;
+  auto fetch_window = [&]() __attribute__((always_inline)) {
+    raw = w0 + lane < p.table_stride ? trow[w0 + lane] : 0;
+    win = (int64_t)((unsigned)raw < (unsigned)p.num_pages ? raw : 0) * page_rows + head_rows;
+  };
+  fetch_window();
+  // row of the cache (head hk) of a 16-row-aligned key of the window
+  auto cache_row = [&](int key) __attribute__((always_inline)) {
+    const int i = min(key >> p.psl, p.table_stride - 1) - w0;
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)win, i);
+    const int hi = __builtin_amdgcn_readlane((int)(win >> 32), i);
+    return (int64_t)(((uint64_t)(uint32_t)hi << 32) | lo) + (key & pmask);
+  };
+  struct Tile {
+    uint4 k[CK == 0 ? 4 : 2];  // 16-bit: [key block][32 dims]; codes: [key block]
+    uint4 v[CK == 0 ? 4 : 2];  // 16-bit: rows 8 i + lane / 8; codes: rows 16 i + lane / 4
+    uint32_t ke[2], ve[2];
+  };
+  auto load_tile = [&](Tile& t, int key0) __attribute__((always_inline)) {  // a tile of the window
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const int64_t at = cache_row(key0 + 16 * kb);
+      if constexpr (CK == 0) {
+        const char* kp = p.page[0] + (at + l16) * 128 + g * 16;
+        t.k[2 * kb] = *reinterpret_cast<const uint4*>(kp);
+        t.k[2 * kb + 1] = *reinterpret_cast<const uint4*>(kp + 64);
+        const char* vp = p.page[1] + (at + (lane >> 3)) * 128 + (lane & 7) * 16;
+        t.v[2 * kb] = *reinterpret_cast<const uint4*>(vp);
+        t.v[2 * kb + 1] = *reinterpret_cast<const uint4*>(vp + 8 * 128);
+      } else {
+        t.k[kb] = *reinterpret_cast<const uint4*>(p.page[0] + (at + l16) * 64 + g * 16);
+        t.ke[kb] = p.exp[0][at + l16];
+        t.v[kb] = *reinterpret_cast<const uint4*>(p.page[1] + (at + (lane >> 2)) * 64 + (lane & 3) * 16);
+        t.ve[kb] = p.exp[1][at + (lane >> 2)];
+      }
+    }
+  };
+
+  constexpr int STEP = 4 * ST;
+  Tile ta, tb;
+  int key = k_begin + wave * ST;
+  // (a window has at least 64 pages of 16 rows: the range's first eight tiles are in it)
+  const bool early = p.seqs == 1 && p.table_stride > 0;
+  if (early) {
+    load_tile(ta, key);
+    if (p.chunk > STEP) load_tile(tb, key + STEP);
+  }
   const int c0 = p.cu[b];
   const int nq = new_tokens(p, c0, p.cu[b + 1]);
   const int len = checked_len(p.kv_lens[b], p.cap, p.fault);
@@ -655,7 +707,7 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
   if (rows == 0) return;
   const int pos0 = len - nq;
   const int lim_lo = key_limit(pos0, len, p.block), lim_hi = key_limit(len - 1, len, p.block);
-  const int k_begin = split * p.chunk, k_end = min(k_begin + p.chunk, lim_hi);
+  const int k_end = min(k_begin + p.chunk, lim_hi);
 
   int limit[RB], tok[RB], head[RB];
 #pragma unroll
@@ -675,16 +727,23 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
     return;
   }
 
-  const int32_t* trow = p.table + (int64_t)b * p.table_stride;
   const int pages = (len + (1 << p.psl) - 1) >> p.psl;
-  const int pmask = (1 << p.psl) - 1;
-  const int64_t page_rows = (int64_t)p.kv_heads << p.psl, head_rows = (int64_t)hk << p.psl;
-  int w0 = k_begin >> p.psl;
-  int win = load_window(p, trow, w0, pages, lane);
-  auto cache_row = [&](int key) __attribute__((always_inline)) {
-    const int lp = min(key >> p.psl, pages - 1);
-    const int page = __builtin_amdgcn_readlane(win, lp - w0);
-    return (int64_t)page * page_rows + head_rows + (key & pmask);
+  auto report_pages = [&]() __attribute__((always_inline)) {
+    if (w0 + lane < pages && (unsigned)raw >= (unsigned)p.num_pages) kv_fault(p.fault);
+  };
+  report_pages();
+  if (!early) {
+    load_tile(ta, key);
+    if (p.chunk > STEP) load_tile(tb, key + STEP);
+  }
+  auto load = [&](Tile& t, int key0) __attribute__((always_inline)) {
+    const int last = min((key0 + ST - 1) >> p.psl, p.table_stride - 1);
+    if (__builtin_expect(last - w0 >= 64, 0)) {
+      w0 = key0 >> p.psl;
+      fetch_window();
+      report_pages();
+    }
+    load_tile(t, key0);
   };
 
   bf16x8 qf[RB][2];
@@ -696,36 +755,6 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
     for (int kk = 0; kk < 2; ++kk)
       qf[rb][kk] = *reinterpret_cast<const bf16x8*>(q + (CK == 0 ? kk * 32 + 8 * g : 16 * g + 8 * kk));
   }
-
-  struct Tile {
-    uint4 k[CK == 0 ? 4 : 2];  // 16-bit: [key block][32 dims]; codes: [key block]
-    uint4 v[CK == 0 ? 4 : 2];  // 16-bit: rows 8 i + lane / 8; codes: rows 16 i + lane / 4
-    uint32_t ke[2], ve[2];
-  };
-  auto load = [&](Tile& t, int key0) __attribute__((always_inline)) {
-    const int last = min((key0 + ST - 1) >> p.psl, pages - 1);
-    if (last - w0 >= 64) {
-      w0 = key0 >> p.psl;
-      win = load_window(p, trow, w0, pages, lane);
-    }
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      const int64_t at = cache_row(key0 + 16 * kb);
-      if constexpr (CK == 0) {
-        const char* kp = p.page[0] + (at + l16) * 128 + g * 16;
-        t.k[2 * kb] = *reinterpret_cast<const uint4*>(kp);
-        t.k[2 * kb + 1] = *reinterpret_cast<const uint4*>(kp + 64);
-        const char* vp = p.page[1] + (at + (lane >> 3)) * 128 + (lane & 7) * 16;
-        t.v[2 * kb] = *reinterpret_cast<const uint4*>(vp);
-        t.v[2 * kb + 1] = *reinterpret_cast<const uint4*>(vp + 8 * 128);
-      } else {
-        t.k[kb] = *reinterpret_cast<const uint4*>(p.page[0] + (at + l16) * 64 + g * 16);
-        t.ke[kb] = p.exp[0][at + l16];
-        t.v[kb] = *reinterpret_cast<const uint4*>(p.page[1] + (at + (lane >> 2)) * 64 + (lane & 3) * 16);
-        t.ve[kb] = p.exp[1][at + (lane >> 2)];
-      }
-    }
-  };
 
   f32x4 o[RB][4];
   float m_ref[RB], l_run[RB];
@@ -845,11 +874,6 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
   };
 
   // two tiles in registers: the loads of one fly while the other is used
-  constexpr int STEP = 4 * ST;
-  Tile ta, tb;
-  int key = k_begin + wave * ST;
-  if (key < k_end) load(ta, key);
-  if (key + STEP < k_end) load(tb, key + STEP);
 #pragma unroll 1
   while (key < k_end) {
     tile_step(ta, key);
@@ -940,29 +964,42 @@ __device__ __forceinline__ void merge_store(const PagedArgs& p, int n, float m, 
 }
 
 // One wave per row: four groups of 16 lanes x 4 columns, group g over the key ranges g, g + 4, ...; 32 ranges' partials
-// are in flight at once, joined in a fixed order.  `first`: the row in its first range's slot, `n`: ranges with a key
-// that the row sees.
+// are in flight at once, joined in a fixed order.  `first`: the row in its first range's slot, `r`: its first 32 ranges'
+// partials, fetched before it is known how many of them the row sees; `n`: that number.
+struct Ranges {
+  float ls[8];
+  f32x4 v[8];
+};
+template <int ROWS>
+__device__ __forceinline__ void load_ranges(const PagedArgs& p, int64_t first, int s0, int lane, Ranges& r) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int s = s0 + 4 * i + (lane >> 4);
+    r.ls[i] = -INFINITY;
+    r.v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (s < p.splits) {
+      const int64_t at = first + (int64_t)s * ROWS;
+      r.ls[i] = p.part_lse[at];
+      r.v[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * HD + (lane & 15) * 4);
+    }
+  }
+}
 template <bool F16, int ROWS>
-__device__ __forceinline__ void merge_row(const PagedArgs& p, int64_t first, int n, int tok, int head, int lane) {
+__device__ __forceinline__ void merge_row(const PagedArgs& p, int64_t first, Ranges& r, int n, int tok, int head,
+                                          int lane) {
   const int d = (lane & 15) * 4, g = lane >> 4;
   float m = -INFINITY, l = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
   for (int s0 = 0; s0 < n; s0 += 32) {
-    float ls[8];
-    f32x4 v[8];
+    if (s0 > 0) load_ranges<ROWS>(p, first, s0, lane, r);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int s = s0 + 4 * i + g;
-      ls[i] = -INFINITY;
-      v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (s < n) {
-        const int64_t at = first + (int64_t)s * ROWS;
-        ls[i] = p.part_lse[at];
-        v[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * HD + d);
+    for (int i = 0; i < 8; ++i)
+      if (s0 + 4 * i + g >= n) {  // a range that the row does not see: never written
+        r.ls[i] = -INFINITY;
+        r.v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
-    }
-    merge_ranges(ls, v, m, l, acc);
+    merge_ranges(r.ls, r.v, m, l, acc);
   }
 #pragma unroll
   for (int o = 16; o < 64; o <<= 1) {
@@ -1026,6 +1063,9 @@ __global__ void __launch_bounds__(NT) attn_paged_merge_step(PagedArgs p) {
   constexpr int RS = RB * 16;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = blockIdx.x / p.kv_heads, hk = blockIdx.x - b * p.kv_heads, r = blockIdx.y * 4 + wave;
+  const int64_t first = (int64_t)blockIdx.x * p.splits * RS + r;
+  Ranges part;
+  load_ranges<RS>(p, first, 0, lane, part);
   const int c0 = p.cu[b];
   const int nq = new_tokens(p, c0, p.cu[b + 1]);
   if (r >= nq * p.group) return;
@@ -1033,8 +1073,7 @@ __global__ void __launch_bounds__(NT) attn_paged_merge_step(PagedArgs p) {
   if (key_limit(len - 1, len, p.block) <= p.chunk) return;  // one range: written where computed
   const int t = r / p.group;
   const int limit = key_limit(len - nq + t, len, p.block);
-  merge_row<F16, RS>(p, (int64_t)blockIdx.x * p.splits * RS + r, (limit + p.chunk - 1) / p.chunk, c0 + t,
-                     hk * p.group + r - t * p.group, lane);
+  merge_row<F16, RS>(p, first, part, (limit + p.chunk - 1) / p.chunk, c0 + t, hk * p.group + r - t * p.group, lane);
 }
 
 // ------------------------------------------------------------------------------------------------ plan
@@ -1109,7 +1148,7 @@ Plan make_plan(const mapa_attn_paged_desc& d) {
       pl.splits = rest ? even_splits(rest, tiles_k, slots, 4.0, 64) : 1;
       if (pl.splits == 1) pl.whole = (int)tasks;
     } else {
-      pl.splits = ragged_splits(tasks, tiles_k, slots, 4.0, 64);
+      pl.splits = ragged_splits(tasks, tiles_k, slots, 12.0, 64);
       if (pl.splits == 1) pl.whole = (int)tasks;
     }
   }
