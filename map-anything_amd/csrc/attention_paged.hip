@@ -156,20 +156,22 @@ __device__ __forceinline__ bf16x8 only(bf16x8 v, int j) {
   return __builtin_bit_cast(bf16x8, r);
 }
 
-// Row tile of the chunk kernel -> (sequence, its first packed row, its new tokens, tile in it), by a wave-wide prefix sum
+// Row tile of the chunk kernel -> (sequence, its first packed row, its new and its cached tokens, tile in it), by a wave-wide prefix sum
 // over the sequences' tile counts, 64 at a time; seq -1: no such tile.
 struct RowTile {
-  int seq, c0, nq, tile;
+  int seq, c0, nq, len, tile;
 };
 __device__ __forceinline__ RowTile find_tile(const PagedArgs& p, int tile, int lane) {
   int before = 0;
 #pragma unroll 1
   for (int s0 = 0; s0 < p.seqs; s0 += 64) {
     const int s = s0 + lane;
-    int q0 = 0, n = 0;
+    int q0 = 0, n = 0, len = 0;
     if (s < p.seqs) {
       q0 = p.cu[s];
+      len = p.kv_lens[s];
       n = new_tokens(p, q0, p.cu[s + 1]);
+      len = checked_len(len, p.cap, p.fault);
     }
     int sum = (n + p.per_tile - 1) / p.per_tile;
     const int own = sum;
@@ -182,11 +184,11 @@ __device__ __forceinline__ RowTile find_tile(const PagedArgs& p, int tile, int l
     if (past) {
       const int l = __builtin_ctzll(past);
       return RowTile{s0 + l, __builtin_amdgcn_readlane(q0, l), __builtin_amdgcn_readlane(n, l),
-                     tile - before - __builtin_amdgcn_readlane(sum - own, l)};
+                     __builtin_amdgcn_readlane(len, l), tile - before - __builtin_amdgcn_readlane(sum - own, l)};
     }
     before += __builtin_amdgcn_readlane(sum, 63);
   }
-  return RowTile{-1, 0, 0, 0};
+  return RowTile{-1, 0, 0, 0, 0};
 }
 // task of the chunk kernel -> (K/V head, row tile): row tiles inside heads (they share K/V), the last ones (the longest
 // key ranges under a causal mask) first
@@ -206,7 +208,7 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
 
   // whole tasks first, each XCD a contiguous run of them; then the split ones, where workgroups that share a K/V range
   // run together on one XCD: (head, range, row tile) if all tasks are split — ranges outermost would give one XCD the
-  // last ranges, which only the longest sequence has (ragged causal chunks: 201 us so, 128 us head by head) — and
+  // last ranges, which only the longest sequence has (ragged causal int8 chunks: 201 us so, 142 us head by head) — and
   // (range, task) for the rest of one sequence's tasks
   int task, split = 0, slot = -1;
   if ((int)blockIdx.x < p.whole) {
@@ -224,10 +226,9 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
   int hk, tile;
   task_coords(p, task, hk, tile);
   const RowTile rt0 = find_tile(p, tile, lane);
-  const int b = rt0.seq, nq = rt0.nq, c0 = rt0.c0;
+  const int b = rt0.seq, nq = rt0.nq, c0 = rt0.c0, len = rt0.len;
   tile = rt0.tile;
   if (b < 0) return;
-  const int len = __builtin_amdgcn_readfirstlane(checked_len(p.kv_lens[b], p.cap, p.fault));
   const int t0 = tile * p.per_tile;                       // first token of the tile, in its sequence
   const int rows = min(p.per_tile, nq - t0) * p.group;    // rows of the tile
   const int pos0 = len - nq + t0;                         // position of the first token
@@ -253,6 +254,13 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
   }
   const int kt0 = k_begin / KT, kt1 = (k_end + KT - 1) / KT;
   const int kt_free = min(lim_lo, k_end) / KT;  // tiles below: every key seen by every row
+
+  bf16x8 qf[4];
+  {
+    const uint16_t* q = p.q + (int64_t)tok * p.qr + head * p.qh;
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) qf[kk] = *reinterpret_cast<const bf16x8*>(q + kk * 16 + 8 * hl);
+  }
 
   // pages
   const int32_t* trow = p.table + (int64_t)b * p.table_stride;
@@ -362,13 +370,6 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
     store8(0, kt0 + 1, P1());
     place(min(kt0 + 2, kt1 - 1), P0());
     fetch8(0, P0());
-  }
-
-  bf16x8 qf[4];
-  {
-    const uint16_t* q = p.q + (int64_t)tok * p.qr + head * p.qh;
-#pragma unroll
-    for (int kk = 0; kk < 4; ++kk) qf[kk] = *reinterpret_cast<const bf16x8*>(q + kk * 16 + 8 * hl);
   }
 
   f32x16 o[2], st[2][2];  // output rows; scores by tile parity
@@ -1024,7 +1025,7 @@ __global__ void __launch_bounds__(NT) attn_paged_merge_chunk(PagedArgs p) {
   task_coords(p, p.whole + j, hk, tile);
   const RowTile rt = find_tile(p, tile, lane);
   if (rt.seq < 0) return;
-  const int len = checked_len(p.kv_lens[rt.seq], p.cap, p.fault);
+  const int len = rt.len;
   const int t0 = rt.tile * p.per_tile, pos0 = len - rt.nq + t0;
   const int rows = min(p.per_tile, rt.nq - t0) * p.group;
   if (key_limit(pos0 + (rows - 1) / p.group, len, p.block) <= p.chunk) return;  // one range: written where computed
