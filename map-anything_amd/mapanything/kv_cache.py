@@ -121,6 +121,9 @@ class PagedKVCache:
                                   f"{heads if heads is not None else 'heads'}, {HEAD_DIM}) with a contiguous head dim")
         if t.device != self.k.device:
             raise nat.NativeError(f"PagedKVCache: {name} is on {t.device}, the pages on {self.k.device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise nat.NativeError(f"PagedKVCache: {name} needs a gradient, and none passes through the cache "
+                                  "(torch.no_grad() or detach())")
 
     def _same(self, batch: KVBatch):
         if batch.table.device != self.k.device:
@@ -163,7 +166,7 @@ class PagedKVCache:
         which hold the new tokens' keys and values already.  Query heads are a multiple of the cache's heads (query
         head h reads head h // (query heads // heads)).  mask_block: 0, a token sees its whole sequence; n, it sees up
         to the end of its block of n positions (1: causal; tokens per view: each view itself and the earlier ones).
-        scale: 1/8 by default.  A token that sees nothing gets zeros and an lse of -inf; rows behind the last sequence
+        scale: 1/8 by default (None or 0).  No gradient passes.  A token that sees nothing gets zeros and an lse of -inf; rows behind the last sequence
         are left as they are.  return_lse: also (query heads, rows) fp32 log-sum-exp, as `_native.attn_merge` takes it.
         """
         self._rows(q, "q")

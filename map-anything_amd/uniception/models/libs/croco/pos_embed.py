@@ -132,6 +132,8 @@ class RoPEAxes:
             if positions.is_floating_point() or positions.is_complex() or positions.dtype == torch.bool:
                 raise ValueError(f"RoPEAxes: positions must be integer or fp32, got {positions.dtype}")
             positions = positions.to(torch.int64)
+        if positions.requires_grad and torch.is_grad_enabled():
+            raise ValueError("RoPEAxes: no gradient passes to the positions")
         if positions.device != tokens.device:
             positions = positions.to(tokens.device)
         needs = torch.is_grad_enabled() and (tokens.requires_grad or (keys is not None and keys.requires_grad))

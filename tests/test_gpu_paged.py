@@ -234,6 +234,11 @@ SHAPES = [
     ([(1370, 2740)], 2, 2, 64),
     ([(5, 100)] * 70, 8, 8, 16),                                    # more sequences than a wave has lanes
     ([(9, 60)] * 70, 16, 2, 16),
+    ([(1, 3000), (2, 1100)], 40, 1, 16),                            # 40 heads of a group: three tokens a tile
+    ([(3, 500), (1, 1)], 128, 1, 64),                               # 128: one token a tile
+    ([(1, 3000), (3, 1024), (2, 1025)], 4, 4, 1024),                # the largest pages
+    ([(150, 2100)], 4, 4, 1024),
+    ([(1, 4000), (1, 2500)] * 30, 8, 8, 16),                        # ranges of more pages than a wave's window holds
 ]
 
 
@@ -280,6 +285,51 @@ def test_attention_paged_scale_strides_and_growing_scores(nat, seqs, heads, kv_h
     want, _, tol, _ = s.expect(q, 0, scale=torch.tensor(0.3, dtype=torch.float32).item())
     ref.within(out, want, tol, "out")
     assert (owide.unflatten(1, (heads, 128))[:, :, :64] == 0).all()
+
+
+@pytest.mark.parametrize("pages", [torch.bfloat16, E4M3], ids=str)
+@pytest.mark.parametrize("seqs,heads,kv_heads,page", [([(1, 9000)], 12, 12, 16), ([(5, 3000), (2, 100)], 6, 2, 32),
+                                                       ([(140, 5000)], 4, 4, 16), ([(33, 40), (70, 2500)], 4, 2, 16)])
+def test_attention_paged_without_workspace(nat, pages, seqs, heads, kv_heads, page):
+    """The C entry without a workspace (or with one too small): every row's keys in one workgroup, over many page windows."""
+    import ctypes
+
+    s = Scene(seqs, kv_heads, page, pages)
+    s.fill(17)
+    q = _randn(s.rows, heads, 64, seed=18, dtype=torch.bfloat16)
+    want, wlse, tol, ltol = s.expect(q, 1)
+    small = torch.empty(64, dtype=torch.uint8, device="cuda")
+    for ws in (None, small):
+        out, lse = torch.empty_like(q), torch.empty(heads, s.rows, device="cuda")
+        d = nat.AttnPagedDesc(cache=s.cache.desc, batch=s.batch._rows(s.rows), dtype=nat.BF16, heads=heads,
+                              q=q.data_ptr(), o=out.data_ptr(), q_rstride=q.stride(0), q_hstride=64,
+                              o_rstride=out.stride(0), o_hstride=64, lse=lse.data_ptr(), mask_block=1)
+        assert nat.lib().mapa_attention_paged_workspace_bytes(ctypes.byref(d)) > 64
+        if ws is not None:
+            d.workspace, d.workspace_bytes = ws.data_ptr(), ws.numel()
+        nat.check(nat.lib().mapa_attention_paged(ctypes.byref(d), nat.stream()), "mapa_attention_paged")
+        ref.within(out, want, tol, "out")
+        ref.within(lse, wlse, ltol, "lse")
+
+
+@pytest.mark.parametrize("block", [1, 37])
+def test_attention_paged_several_streams_at_once(nat, block):
+    """Calls of different shapes in flight on three streams at once: each has partials of its own."""
+    work = []
+    for i, seqs in enumerate(([(1, 9000)], [(200, 3000), (40, 600)], [(3, 800)] * 9)):
+        s = Scene(seqs, 4, 32, torch.bfloat16, seed=i)
+        s.fill(60 + i)
+        q = _randn(s.rows, 8, 64, seed=70 + i, dtype=torch.bfloat16)
+        work.append((s, q, s.cache.attend(q, s.batch, mask_block=block), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        outs = []
+        for s, q, _, st in work:
+            with torch.cuda.stream(st):
+                outs.append([s.cache.attend(q, s.batch, mask_block=block) for _ in range(4)])
+        torch.cuda.synchronize()
+        for (_, _, want, _), got in zip(work, outs):
+            assert all(torch.equal(o, want) for o in got)
 
 
 @pytest.mark.parametrize("pages", [torch.bfloat16, E4M3, torch.int8], ids=str)
@@ -488,6 +538,12 @@ def test_paged_class_refusals(nat):
     for k, v in ((q, q.float()), (q.double(), q.double()), (q, q[:0])):
         with pytest.raises(nat.NativeError):
             s.cache.write(k, v, s.batch)
+    g = q.clone().requires_grad_()
+    for call in (lambda: s.cache.attend(g, s.batch), lambda: s.cache.write(g, q, s.batch)):
+        with pytest.raises(nat.NativeError):
+            call()
+        with torch.no_grad():
+            call()
     with pytest.raises(nat.NativeError):
         s.cache.attend(q, s.batch, out=q.float())
     with pytest.raises(nat.NativeError):

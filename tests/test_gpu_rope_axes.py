@@ -190,6 +190,8 @@ def test_rope_axes_empty_and_refused(RoPEAxes):
     with pytest.raises(ValueError):
         r(x, pos.double())
     with pytest.raises(ValueError):
+        r(x, pos.float().requires_grad_())
+    with pytest.raises(ValueError):
         r(x[..., ::2], pos)
     with pytest.raises(ValueError):
         r(x[:, :1].expand(1, 2, 4, 64), pos, inplace=True)
