@@ -538,7 +538,9 @@ int mapa_kv_cache_read(const mapa_kv_cache* c, const mapa_kv_batch* b, const int
 
 /* Attention of the batch's new tokens over their sequences' pages (head dim 64), the paged form of mapa_attention.
  * q / o [new_rows][heads][64] bf16 or f16, element strides of row and head; `heads` is a multiple of the cache's heads
-X * A query at position p (of kv_lens[b]) sees keys below: kv_lens[b] (mask_block 0), or the end of p's block of
+ * (query head h reads K/V head h / (heads / cache heads)).  16-bit pages have q's type; values of 8-bit pages that it
+ * does not reach (fp16: from 65520 on) are infinities.
+ * A query at position p (of kv_lens[b]) sees keys below: kv_lens[b] (mask_block 0), or the end of p's block of
  * mask_block positions, (p / mask_block + 1) * mask_block, where that is less (1: causal; tokens per view: every view
  * sees itself and the earlier ones).  A query that sees nothing (more new tokens than cached ones) gets o = 0,
  * lse = -inf.  A query's output depends on the keys and values it sees alone, whatever the hidden rows hold.
