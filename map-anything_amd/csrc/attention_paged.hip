@@ -27,7 +27,7 @@ namespace {
 using namespace mapa_paged;
 
 constexpr int NT = 256;
-constexpr int QB = 128;  // rows of a chunk workgroup
+constexpr int MAX_GROUP = 128;  // query heads per K/V head
 constexpr int KT = 64;   // keys of a chunk tile
 constexpr int ST = 32;   // keys of a step tile
 constexpr float LOG2E = 1.4426950408889634f;
@@ -55,6 +55,7 @@ struct PagedArgs {
   int whole;     // tasks [0, whole) of the chunk kernel walk all their keys, the others are split
   int tiles;     // row tiles of the grid (upper bound)
   int per_tile;  // tokens of a row tile
+  int slot_rows; // rows of a chunk slot
 };
 
 typedef short s4v __attribute__((ext_vector_type(4)));
@@ -198,9 +199,12 @@ __device__ __forceinline__ void task_coords(const PagedArgs& p, int task, int& h
 }
 
 // ------------------------------------------------------------------------------------------------ chunk
-// CK: 0 = 16-bit pages of the query's type, 1 = e4m3, 2 = int8
-template <bool F16, int CK>
-__global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
+// CK: 0 = 16-bit pages of the query's type, 1 = e4m3, 2 = int8.  NW: waves of a workgroup, 32 rows each (the plan's rule
+// and both sides' figures are at chunk_waves).
+template <bool F16, int CK, int NW>
+__global__ void __launch_bounds__(NW * 64, 2) attn_paged_chunk(PagedArgs p) {
+  constexpr int QB = NW * 32;
+  constexpr int PIECES = 8 / NW;  // 8-row pieces of a 64-row tile per wave
   constexpr int TILE = KT * 128;  // 64 rows x 128 B
   __shared__ __attribute__((aligned(1024))) char lds[2 * 2 * TILE];  // K by tile parity, then V
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -293,12 +297,13 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
   // Staging.  A tile's K is needed one step before its V, so step t brings K of tile t + 2 and V of tile t; the V rows'
   // place in the cache is K's of two steps ago (`at`, by tile parity).  Tile numbers past the range are clamped: what
   // they bring is not used.
-  //  * 16-bit pages: a wave moves rows 8 wave and 32 + 8 wave .. + 7 of the tile (8 rows x 128 B lie in one page: a
-  //    scalar base and a fixed offset per lane), the 16-B column XOR-swizzled on the source so that the LDS image stays
-  //    lane-linear.  V's buffer ends where the sequence does, so that rows past it arrive as zeros: whatever their memory
-  //    holds must not meet a zero probability (hidden scores are replaced, so K needs no such care).
-  //  * 8-bit pages: thread -> tile row tid / 4, 16 codes, fetched a step earlier and decoded on the way into LDS.
-  constexpr int NA = CK == 0 ? 2 : 1;  // cache rows to remember per tile
+  //  * 16-bit pages: a wave moves 8-row pieces of K and of V (8 rows x 128 B lie in one page: a scalar base and a fixed
+  //    offset per lane), the 16-B column XOR-swizzled on the source so that the LDS image stays lane-linear.  V's buffer
+  //    ends where the sequence does, so that rows past it arrive as zeros: whatever their memory holds must not meet a
+  //    zero probability (hidden scores are replaced, so K needs no such care).
+  //  * 8-bit pages: four waves take a tile's 64 rows, four lanes a row of 16 codes each, fetched a step earlier and
+  //    decoded on the way into LDS; of eight waves, four take K and four V.
+  constexpr int NA = CK == 0 ? PIECES : 1;  // cache rows to remember per tile
   int64_t at[2][NA];
   const int prow8 = lane >> 3;
   const int koff = prow8 * 128 + (((lane & 7) ^ (((wave & 1) * 4 + (lane >> 4)) & 7)) << 4);
@@ -308,14 +313,14 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
     const int key0 = kt * KT;
     need_window(key0);
 #pragma unroll
-    for (int i = 0; i < NA; ++i) at[par][i] = cache_row(key0 + (CK == 0 ? (i * 4 + wave) * 8 : wave * 16));
+    for (int i = 0; i < NA; ++i) at[par][i] = cache_row(key0 + (CK == 0 ? (i * NW + wave) * 8 : (wave & 3) * 16));
   };
   const uint32_t lds_base = (uint32_t)(uintptr_t)(lds_ptr_t)lds;
   auto dma = [&](auto x_tag, int kt, auto par_tag, auto full_tag) __attribute__((always_inline)) {  // x: 0 K, 1 V
     constexpr int x = decltype(x_tag)::value, par = decltype(par_tag)::value;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int k8 = (i * 4 + wave) * 8;
+    for (int i = 0; i < PIECES; ++i) {
+      const int k8 = (i * NW + wave) * 8;
       int bytes = 1024;
       if constexpr (x == 1 && !decltype(full_tag)::value) {
         const int rows_left = len - kt * KT - k8;
@@ -328,23 +333,29 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
   };
   uint4 creg[2] = {};
   uint32_t ereg[2] = {};
-  auto fetch8 = [&](int x, auto par_tag) __attribute__((always_inline)) {
+  // x: 0 K, 1 V; r: register set
+  auto fetch8 = [&](int x, int r, auto par_tag) __attribute__((always_inline)) {
     constexpr int par = decltype(par_tag)::value;
-    creg[x] = reinterpret_cast<const uint4*>(p.page[x] + at[par][0] * 64)[lane];
-    ereg[x] = (p.exp[x] + at[par][0])[lane >> 2];
+    const char* page = x == 0 ? p.page[0] : p.page[1];
+    const uint8_t* exp = x == 0 ? p.exp[0] : p.exp[1];
+    creg[r] = reinterpret_cast<const uint4*>(page + at[par][0] * 64)[lane];
+    ereg[r] = (exp + at[par][0])[lane >> 2];
   };
-  auto store8 = [&](int x, int kt, auto par_tag) __attribute__((always_inline)) {
+  auto store8 = [&](int x, int r, int kt, auto par_tag) __attribute__((always_inline)) {
     constexpr int par = decltype(par_tag)::value;
     char* dst = lds + (2 * x + par) * TILE;
-    const int row = tid >> 2, ch = (lane & 3) * 2;
-    const float s = exponent_value(ereg[x]);
-    bf16x8 lo = decode8<F16, CK == 2>(uint2{creg[x].x, creg[x].y}, s);
-    bf16x8 hi = decode8<F16, CK == 2>(uint2{creg[x].z, creg[x].w}, s);
+    const int row = (tid & 255) >> 2, ch = (lane & 3) * 2;
+    const float s = exponent_value(ereg[r]);
+    bf16x8 lo = decode8<F16, CK == 2>(uint2{creg[r].x, creg[r].y}, s);
+    bf16x8 hi = decode8<F16, CK == 2>(uint2{creg[r].z, creg[r].w}, s);
     if (kt * KT + row >= len) lo = hi = bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
     const int sw = x == 0 ? (row >> 1) & 7 : ((row >> 1) & 1) << 2;
     *reinterpret_cast<bf16x8*>(dst + row * 128 + ((ch ^ sw) << 4)) = lo;
     *reinterpret_cast<bf16x8*>(dst + row * 128 + (((ch + 1) ^ sw) << 4)) = hi;
   };
+  // eight waves: this wave's tensor, and its tile that step t stores (K t + 2, V t) and fetches (one further)
+  const int mine = wave >> 2;
+  auto tile_of = [&](int t) __attribute__((always_inline)) { return mine == 0 ? t + 2 : t; };
   using T_ = std::integral_constant<bool, true>;
   using F_ = std::integral_constant<bool, false>;
   using P0 = std::integral_constant<int, 0>;
@@ -361,15 +372,25 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
     dma(P0(), kt0, P0(), F_());
     place(min(kt0 + 1, kt1 - 1), P1());
     dma(P0(), kt0 + 1, P1(), F_());
-  } else {
-    fetch8(0, P0());
-    store8(0, kt0, P0());
+  } else if constexpr (NW == 4) {
+    fetch8(0, 0, P0());
+    store8(0, 0, kt0, P0());
     place(min(kt0 + 1, kt1 - 1), P1());
-    fetch8(0, P1());
-    fetch8(1, P0());
-    store8(0, kt0 + 1, P1());
+    fetch8(0, 0, P1());
+    fetch8(1, 1, P0());
+    store8(0, 0, kt0 + 1, P1());
     place(min(kt0 + 2, kt1 - 1), P0());
-    fetch8(0, P0());
+    fetch8(0, 0, P0());
+  } else {
+    if (mine == 0) {
+      fetch8(0, 0, P0());
+      place(min(kt0 + 1, kt1 - 1), P1());
+      fetch8(0, 1, P1());
+      store8(0, 0, kt0, P0());
+      store8(0, 1, kt0 + 1, P1());
+    }
+    place(min(tile_of(kt0), kt1 - 1), P0());
+    fetch8(mine, 0, P0());
   }
 
   f32x16 o[2], st[2][2];  // output rows; scores by tile parity
@@ -480,11 +501,17 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_chunk(PagedArgs p) {
       place(min(t + 2, kt1 - 1), par_tag);
       dma(P0(), t + 2, par_tag, F_());
     } else {
-      store8(1, t, par_tag);
-      store8(0, t + 2, par_tag);
-      fetch8(1, PN());
-      place(min(t + 3, kt1 - 1), PN());
-      fetch8(0, PN());
+      if constexpr (NW == 4) {
+        store8(1, 1, t, par_tag);
+        store8(0, 0, t + 2, par_tag);
+        fetch8(1, 1, PN());
+        place(min(t + 3, kt1 - 1), PN());
+        fetch8(0, 0, PN());
+      } else {
+        store8(mine, 0, tile_of(t), par_tag);
+        place(min(tile_of(t + 1), kt1 - 1), PN());
+        fetch8(mine, 0, PN());
+      }
     }
     if constexpr (MASK) hide(s, t);
     if constexpr (FIRST) m_ref = fmaxf(row_max(s), -1e38f);  // finite also for a row that sees none of the range
@@ -1015,7 +1042,7 @@ __device__ __forceinline__ void merge_row(const PagedArgs& p, int64_t first, Ran
   if (g == 0) merge_store<F16>(p, n, m, l, acc, tok, head, d);
 }
 
-// The split tasks of the chunk kernel: blockIdx.x = task, blockIdx.y = 32 of its 128 rows; 16 lanes x 4 columns per row
+// The split tasks of the chunk kernel: blockIdx.x = task, blockIdx.y = 32 of its rows; 16 lanes x 4 columns per row
 // (there are many rows, so nothing is gained by spreading a row's ranges over lanes)
 template <bool F16>
 __global__ void __launch_bounds__(NT) attn_paged_merge_chunk(PagedArgs p) {
@@ -1035,7 +1062,7 @@ __global__ void __launch_bounds__(NT) attn_paged_merge_chunk(PagedArgs p) {
     if (r >= rows) return;
     const int t = r / p.group, tok = rt.c0 + t0 + t, head = hk * p.group + r - t * p.group;
     const int n = (key_limit(pos0 + t, len, p.block) + p.chunk - 1) / p.chunk;
-    const int64_t first = (int64_t)j * p.splits * QB + r;
+    const int64_t first = (int64_t)j * p.splits * p.slot_rows + r;
     float m = -INFINITY, l = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
@@ -1047,7 +1074,7 @@ __global__ void __launch_bounds__(NT) attn_paged_merge_chunk(PagedArgs p) {
         ls[k] = -INFINITY;
         v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (s0 + k < n) {
-          const int64_t at = first + (int64_t)(s0 + k) * QB;
+          const int64_t at = first + (int64_t)(s0 + k) * p.slot_rows;
           ls[k] = p.part_lse[at];
           v[k] = *reinterpret_cast<const f32x4*>(p.part_o + at * HD + d);
         }
@@ -1079,7 +1106,9 @@ __global__ void __launch_bounds__(NT) attn_paged_merge_step(PagedArgs p) {
 
 // ------------------------------------------------------------------------------------------------ plan
 struct Plan {
-  int rb;  // row blocks of the step kernel (0: the chunk kernel)
+  int rb;     // row blocks of the step kernel (0: the chunk kernel)
+  int waves;  // of a chunk workgroup
+  int slot_rows;
   int tiles, per_tile;
   int whole, splits, chunk;
   int64_t slots;  // workgroups that leave partials
@@ -1120,23 +1149,38 @@ int ragged_splits(int64_t tasks, int tiles, int slots, double fixed, int most) {
   return std::max(1, std::min({most, tiles, (int)(n + 0.5)}));
 }
 
+// Waves of a chunk workgroup (32 rows each).  Eight share a tile's decoding where two workgroups of four do it twice: an
+// 8-view chunk over int8 pages takes 779 us with eight and 860 with four (e4m3 739 and 765), a 1370-token view over 100
+// views 737 and 793 (702 and 713) though a twelfth of its eight-wave rows is empty.  16-bit pages have nothing to decode
+// (695 and 701 us, 676 and 670), and ragged batches want the finer pieces (ragged causal int8 chunks 134 and 121 us).
+int chunk_waves(const mapa_attn_paged_desc& d) {
+  const bool codes = d.cache.dtype == MAPA_FP8 || d.cache.dtype == MAPA_I8;
+  const int64_t rows = (int64_t)d.batch.max_new * (d.heads / d.cache.heads);
+  const int64_t four = (rows + 127) / 128 * 128, eight = (rows + 255) / 256 * 256;
+  return codes && d.batch.seqs == 1 && eight * 10 <= four * 11 ? 8 : 4;
+}
+
 Plan make_plan(const mapa_attn_paged_desc& d) {
   Plan pl = {};
   const int group = d.heads / d.cache.heads;
   const int cap = kv_cap(d.cache, d.batch);
   const int64_t rows = (int64_t)d.batch.max_new * group;
-  const int slots = 2 * cu_count();  // resident workgroups
+  int slots = 2 * cu_count();  // resident workgroups
   int unit, tiles_k;
   int64_t tasks;
   if (rows <= 32) {
     pl.rb = rows <= 16 ? 1 : 2;
+    pl.slot_rows = 16 * pl.rb;
     tasks = (int64_t)d.batch.seqs * d.cache.heads;
     unit = 4 * ST;
     tiles_k = std::max(1, (cap + unit - 1) / unit);
     pl.splits = d.batch.seqs == 1 ? even_splits(tasks, tiles_k, slots, 4.0, 128)
                                   : ragged_splits(tasks, tiles_k, slots, 4.0, 128);
   } else {
-    pl.per_tile = std::max(1, QB / group);
+    pl.waves = chunk_waves(d);
+    if (pl.waves == 8) slots /= 2;
+    pl.slot_rows = pl.waves * 32;
+    pl.per_tile = std::max(1, pl.slot_rows / group);
     const int64_t a = (int64_t)d.batch.new_rows / pl.per_tile + d.batch.seqs;
     const int64_t b = (int64_t)d.batch.seqs * ((d.batch.max_new + pl.per_tile - 1) / pl.per_tile);
     pl.tiles = (int)std::min(a, b);
@@ -1157,7 +1201,7 @@ Plan make_plan(const mapa_attn_paged_desc& d) {
   pl.splits = (tiles_k + per - 1) / per;
   pl.chunk = per * unit;
   pl.slots = pl.splits > 1 ? (tasks - pl.whole) * pl.splits : 0;
-  pl.ws = pl.slots * (pl.rb ? 16 * pl.rb : QB) * (HD + 1) * 4;
+  pl.ws = pl.slots * pl.slot_rows * (HD + 1) * 4;
   return pl;
 }
 // the same work without a workspace: every task walks all its keys
@@ -1177,7 +1221,7 @@ int check_desc(const mapa_attn_paged_desc* d) {
   MAPA_CHECK_ARG(d->cache.dtype == MAPA_FP8 || d->cache.dtype == MAPA_I8 || d->cache.dtype == d->dtype,
                  "%s: 16-bit pages must have the queries' type", who);
   MAPA_CHECK_ARG(d->heads > 0 && d->heads <= 65535 && d->heads % d->cache.heads == 0 &&
-                     d->heads / d->cache.heads <= QB,
+                     d->heads / d->cache.heads <= MAX_GROUP,
                  "%s: %d query heads over %d K/V heads", who, d->heads, d->cache.heads);
   MAPA_CHECK_ARG(d->mask_block >= 0, "%s: bad mask_block %d", who, d->mask_block);
   MAPA_CHECK_ARG(d->scale >= 0.f && d->scale < 1e30f, "%s: bad scale %g", who, (double)d->scale);
@@ -1186,7 +1230,9 @@ int check_desc(const mapa_attn_paged_desc* d) {
 
 template <bool F16, int CK>
 void launch(const PagedArgs& a, const Plan& pl, unsigned grid, hipStream_t stream) {
-  if (pl.rb == 0) hipLaunchKernelGGL((attn_paged_chunk<F16, CK>), dim3(grid), dim3(NT), 0, stream, a);
+  if (CK != 0 && pl.rb == 0 && pl.waves == 8)
+    hipLaunchKernelGGL((attn_paged_chunk<F16, CK, CK != 0 ? 8 : 4>), dim3(grid), dim3(512), 0, stream, a);
+  else if (pl.rb == 0) hipLaunchKernelGGL((attn_paged_chunk<F16, CK, 4>), dim3(grid), dim3(256), 0, stream, a);
   else if (pl.rb == 1) hipLaunchKernelGGL((attn_paged_step<F16, CK, 1>), dim3(grid), dim3(NT), 0, stream, a);
   else hipLaunchKernelGGL((attn_paged_step<F16, CK, 2>), dim3(grid), dim3(NT), 0, stream, a);
 }
@@ -1198,7 +1244,7 @@ int launch_all(const PagedArgs& a, const Plan& pl, int page_dtype, int64_t wgs, 
   MAPA_CHECK_LAUNCH("mapa_attention_paged");
   if (pl.slots == 0) return 0;
   if (pl.rb == 0) {
-    const dim3 grid(a.tiles * a.kv_heads - a.whole, QB / 32);
+    const dim3 grid(a.tiles * a.kv_heads - a.whole, a.slot_rows / 32);
     hipLaunchKernelGGL((attn_paged_merge_chunk<F16>), grid, dim3(NT), 0, stream, a);
   } else {
     const dim3 grid(a.seqs * a.kv_heads, (std::min(a.max_new * a.group, 16 * pl.rb) + 3) / 4);
@@ -1239,12 +1285,13 @@ extern "C" int mapa_attention_paged(const mapa_attn_paged_desc* d, hipStream_t s
   a.heads = d->heads; a.kv_heads = d->cache.heads; a.group = d->heads / d->cache.heads;
   a.block = d->mask_block;
   a.splits = pl.splits; a.chunk = pl.chunk; a.whole = pl.whole; a.tiles = pl.tiles; a.per_tile = pl.per_tile;
+  a.slot_rows = pl.slot_rows;
   const int64_t wgs = pl.rb ? (int64_t)b.seqs * a.kv_heads * a.splits : pl.whole + pl.slots;
   MAPA_CHECK_ARG(wgs <= 0x7fffffff && (int64_t)pl.tiles * a.kv_heads <= 0x7fffffff,
                  "mapa_attention_paged: too many workgroups");
   if (pl.slots) {
     a.part_o = (float*)d->workspace;
-    a.part_lse = a.part_o + pl.slots * (pl.rb ? 16 * pl.rb : QB) * HD;
+    a.part_lse = a.part_o + pl.slots * pl.slot_rows * HD;
   }
   return d->dtype == MAPA_F16 ? launch_all<true>(a, pl, d->cache.dtype, wgs, stream)
                               : launch_all<false>(a, pl, d->cache.dtype, wgs, stream);

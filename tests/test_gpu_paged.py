@@ -232,6 +232,8 @@ SHAPES = [
     ([(45, 2500)], 15, 5, 16),                                      # three heads of a group: 126 of a tile's 128 rows
     ([(300, 5000)], 12, 12, 64),
     ([(1370, 2740)], 2, 2, 64),
+    ([(250, 1111)], 4, 4, 16),                                      # one sequence that fills workgroups of 256 rows
+    ([(500, 3000)], 2, 1, 32),
     ([(5, 100)] * 70, 8, 8, 16),                                    # more sequences than a wave has lanes
     ([(9, 60)] * 70, 16, 2, 16),
     ([(1, 3000), (2, 1100)], 40, 1, 16),                            # 40 heads of a group: three tokens a tile
