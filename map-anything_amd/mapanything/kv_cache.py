@@ -115,9 +115,10 @@ class PagedKVCache:
                                     None if v_exp is None else v_exp.data_ptr())
 
     def _rows(self, t: torch.Tensor, name: str, heads: Optional[int] = None):
-        if t.ndim != 3 or t.shape[2] != HEAD_DIM or (heads is not None and t.shape[1] != heads) or \
-                (t.numel() and t.stride(2) != 1):
-            raise nat.NativeError(f"PagedKVCache: {name} {tuple(t.shape)} must be (rows, "
+        shape = t.shape
+        if len(shape) != 3 or shape[2] != HEAD_DIM or (heads is not None and shape[1] != heads) or \
+                (t.stride(2) != 1 and t.numel()):
+            raise nat.NativeError(f"PagedKVCache: {name} {tuple(shape)} must be (rows, "
                                   f"{heads if heads is not None else 'heads'}, {HEAD_DIM}) with a contiguous head dim")
         if t.device != self.k.device:
             raise nat.NativeError(f"PagedKVCache: {name} is on {t.device}, the pages on {self.k.device}")
@@ -150,12 +151,14 @@ class PagedKVCache:
             raise nat.NativeError(f"PagedKVCache: cu_rows {tuple(cu_rows.shape)} does not fit the batch")
         heads = self.k.shape[1]
         if out is None:
-            out = tuple(batch.table.new_empty(rows, heads, HEAD_DIM, dtype=dtype) for _ in range(2))
-        k, v = out
-        for t, name in ((k, "k"), (v, "v")):
-            self._rows(t, name, heads)
-            if t.shape[0] != rows or t.dtype != k.dtype:
-                raise nat.NativeError(f"PagedKVCache: out must hold {rows} rows of one dtype")
+            shape = (rows, heads, HEAD_DIM)
+            k, v = self.k.new_empty(shape, dtype=dtype), self.k.new_empty(shape, dtype=dtype)
+        else:
+            k, v = out
+            for t, name in ((k, "k"), (v, "v")):
+                self._rows(t, name, heads)
+                if t.shape[0] != rows or t.dtype != k.dtype:
+                    raise nat.NativeError(f"PagedKVCache: out must hold {rows} rows of one dtype")
         with nat.on_device(self.k.device):
             nat.kv_cache_read(self.desc, batch.desc, cu_rows, rows, k, v)
         return k, v
@@ -172,7 +175,7 @@ class PagedKVCache:
         self._rows(q, "q")
         self._same(batch)
         if out is None:
-            out = q.new_empty(q.shape)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
             self._rows(out, "out", q.shape[1])
             if out.shape[0] != q.shape[0] or out.dtype != q.dtype:
