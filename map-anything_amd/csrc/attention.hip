@@ -694,7 +694,7 @@ int64_t sk_workspace_bytes(int slots) { return (int64_t)slots * SK_QBLK * (64 + 
 }  // namespace
 
 extern "C" int64_t mapa_attention_workspace_bytes(const mapa_attn_desc* d) {
-  if (!d || d->dtype != MAPA_BF16) return 0;
+  if (!d || d->dtype == MAPA_F32) return 0;  // both 16-bit types run the split kernel
   return sk_workspace_bytes(sk_slots());
 }
 
