@@ -464,7 +464,7 @@ int mapa_rope2d(void* tokens, int dtype, int B, int H, int N, int D, int64_t sb,
 /* ---------------------------------------------------------------------------------------------------------
  * Rotary positions with several axes (time, row, column, ...): the general form of mapa_rope2d, out of place or in
  * place, forward and backward, one or two tensors (queries and keys) in one launch.
- * Tensor i (i < 2, x[i] may be NULL): x[i] -> y[i] (equal pointers AND strides: in place), shape (batch, heads[i] <= 2048,
+ * Tensor i (i < 2, x[i] may be NULL): x[i] -> y[i] (equal pointers AND strides: in place; the two y share nothing), shape (batch, heads[i] <= 2048,
  * tokens, head_dim), element strides (b, h, n), contiguous head dim.  section[a] pairs belong to axis a; with
  * S = sum(section), 2 S <= head_dim, the dims from 2 S on are copied.  Pair i (axis a, its j-th pair) turns by
  * positions[b][n][a] * freq[i] radians (the angle is reduced in 64 bits): u' = u cos - v sin, v' = v cos + u sin;
@@ -510,7 +510,7 @@ int mapa_rope_axes(const mapa_rope_axes_desc* d, mapa_stream_t stream);
  * tokens / cached tokens.  All three arrays are int32 device memory; what they hold is checked on the device
  * (MAPA_FAULT_KV_RANGE).
  * mapa_kv_cache_write: new rows k, v (f32 / bf16 / f16; element strides of row and head, contiguous 64) into their
- *   pages.  Two sequences must not share a page that the call writes.
+ *   pages.  A page that the call writes stands in the table once (two tokens of one place: either's row).
  * mapa_kv_cache_read: positions 0 .. cu_rows[b + 1] - cu_rows[b] - 1 of every sequence to the packed rows from
  *   cu_rows[b] on (k_out, v_out [rows][heads][64] with element strides, f32 / bf16 / f16); positions past kv_lens[b]
  *   read as zero, rows from cu_rows[seqs] on are left as they are. */

@@ -6,7 +6,9 @@
 // at all row offsets at once (thread i holds the interval of sequence i: one trip to memory however many sequences
 // there are, where a binary search makes log2 of them) and one thread per token looks its page up.  The rows follow as
 // (K or V, head, token): a wave's eight rows are neighbours in the page (512 B of 8-bit codes and eight exponent bytes
-// in a row), where (token, head) order scatters them over eight heads' parts of it.
+// in a row), where (token, head) order scatters them over eight heads' parts of it.  Measured: 25 thousand tokens of 16
+// heads into int8 pages, 153 MB, 36.7 us (4.2 TB/s), 59 thousand back out of them, 365 MB, 80.8 us (4.5 TB/s; copy: 5.04);
+// 32 tokens of 12 heads, 3.4 us, which is a launch and the three trips to memory of offsets, table and rows.
 #include <type_traits>
 
 #include "paged.h"

@@ -7,7 +7,9 @@
 // access where sections and strides allow.  A thread keeps its group of pairs for all of its items, so an item costs
 // one small division and two LDS address lookups beside its loads.  The angle is formed and reduced to a fraction of a turn in 64 bits (a
 // far time times a frequency of one keeps no fraction in 32), then sincospif; per token that is S of them against
-// 2 * heads * S values moved.
+// 2 * heads * S values moved.  Measured: queries and keys of 137 thousand tokens, 12 heads each, bf16, 845 MB in 164 us
+// (5.15 TB/s; copy: 5.04), of 11 thousand, 15 us (4.5), of 16 alone, 4.3 us; eight items in flight per thread, 16 tokens
+// per workgroup and non-temporal accesses were no faster.
 #include "mapa_common.h"
 
 namespace {
@@ -265,6 +267,7 @@ extern "C" int mapa_rope_axes(const mapa_rope_axes_desc* d, hipStream_t stream) 
     in_place = in_place && same;
   }
   if (total == 0 || heads == 0) return 0;
+  MAPA_CHECK_ARG(!a.heads[0] || !a.heads[1] || a.y[0] != a.y[1], "mapa_rope_axes: both tensors have one output");
   MAPA_CHECK_ARG(d->positions != nullptr, "mapa_rope_axes: null positions");
   MAPA_CHECK_ARG(total <= (int64_t)0x7fffffff, "mapa_rope_axes: too many tokens");
   const int size = d->dtype == MAPA_F32 ? 4 : 2;

@@ -18,6 +18,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _native as nat
 
@@ -38,9 +39,16 @@ class KVBatch:
     table (seqs, columns): page of every page_size tokens of a sequence; kv_lens (seqs,): tokens in the cache with the
     new ones; cu_new (seqs + 1,): the packed rows cu_new[b] .. cu_new[b + 1] - 1 are sequence b's new tokens, its last
     positions.  max_new / max_kv: upper bounds of the new / cached tokens of one sequence, which size the launch; left
-    out, they are read from the device (a synchronisation, so not while a graph is captured)."""
+    out, they are read from the device (a synchronisation, so not while a graph is captured).  The tensors' contents may
+    change from call to call; other tensors or bounds make another KVBatch."""
 
-    __slots__ = ("table", "kv_lens", "cu_new", "max_new", "max_kv", "desc")
+    __slots__ = ("_table", "_kv_lens", "_cu_new", "_max_new", "_max_kv", "desc")
+
+    table = property(lambda self: self._table)
+    kv_lens = property(lambda self: self._kv_lens)
+    cu_new = property(lambda self: self._cu_new)
+    max_new = property(lambda self: self._max_new)
+    max_kv = property(lambda self: self._max_kv)
 
     def __init__(self, table: torch.Tensor, kv_lens: torch.Tensor, cu_new: torch.Tensor, *,
                  max_new: Optional[int] = None, max_kv: Optional[int] = None):
@@ -57,7 +65,7 @@ class KVBatch:
             max_new = int((cu_new[1:] - cu_new[:-1]).max()) if seqs else 0
         if max_kv is None:
             max_kv = int(kv_lens.max()) if seqs else 0
-        self.table, self.kv_lens, self.cu_new, self.max_new, self.max_kv = table, kv_lens, cu_new, max_new, max_kv
+        self._table, self._kv_lens, self._cu_new, self._max_new, self._max_kv = table, kv_lens, cu_new, max_new, max_kv
         # a one-row table's stride says nothing, its width does
         width = table.shape[1]
         if seqs > 1 and table.stride(0) != width:
@@ -74,9 +82,15 @@ class KVBatch:
 class PagedKVCache:
     """Pages of keys and values: `k`, `v` (num_pages, heads, page_size, 64) in bf16, fp16, e4m3 (torch.float8_e4m3fn)
     or int8; the 8-bit types carry one exponent byte per row in `k_exp`, `v_exp` (num_pages, heads, page_size) (value =
-    code * 2^(byte - 127), see include/mapa.h).  page_size: a power of two, 16 to 1024."""
+    code * 2^(byte - 127), see include/mapa.h).  page_size: a power of two, 16 to 1024.  The tensors are the cache's
+    for its life: their contents may be moved or filled, larger ones make another cache (wrap)."""
 
-    __slots__ = ("k", "v", "k_exp", "v_exp", "desc")
+    __slots__ = ("_k", "_v", "_k_exp", "_v_exp", "desc")
+
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    k_exp = property(lambda self: self._k_exp)
+    v_exp = property(lambda self: self._v_exp)
 
     def __init__(self, num_pages: int, page_size: int = 64, heads: int = 12, dtype: torch.dtype = torch.bfloat16,
                  device="cuda"):
@@ -109,7 +123,7 @@ class PagedKVCache:
             for e in (k_exp, v_exp):
                 if e.dtype != torch.uint8 or e.shape != k.shape[:3] or not e.is_contiguous() or e.device != k.device:
                     raise nat.NativeError("PagedKVCache: exponents must be contiguous uint8 (pages, heads, page_size)")
-        self.k, self.v, self.k_exp, self.v_exp = k, v, k_exp, v_exp
+        self._k, self._v, self._k_exp, self._v_exp = k, v, k_exp, v_exp
         self.desc = nat.KVCacheDesc(code, k.shape[1], k.shape[2], k.shape[0], k.data_ptr(), v.data_ptr(),
                                     None if k_exp is None else k_exp.data_ptr(),
                                     None if v_exp is None else v_exp.data_ptr())
@@ -120,26 +134,33 @@ class PagedKVCache:
                 (t.stride(2) != 1 and t.numel()):
             raise nat.NativeError(f"PagedKVCache: {name} {tuple(shape)} must be (rows, "
                                   f"{heads if heads is not None else 'heads'}, {HEAD_DIM}) with a contiguous head dim")
-        if t.device != self.k.device:
-            raise nat.NativeError(f"PagedKVCache: {name} is on {t.device}, the pages on {self.k.device}")
+        if t.device != self._k.device:
+            raise nat.NativeError(f"PagedKVCache: {name} is on {t.device}, the pages on {self._k.device}")
         if t.requires_grad and torch.is_grad_enabled():
             raise nat.NativeError(f"PagedKVCache: {name} needs a gradient, and none passes through the cache "
                                   "(torch.no_grad() or detach())")
 
+    def _out(self, t: torch.Tensor, name: str, heads: int):
+        self._rows(t, name, heads)
+        if (t.shape[0] > 1 and t.stride(0) == 0) or (heads > 1 and t.stride(1) == 0):
+            raise nat.NativeError(f"PagedKVCache: {name} is expanded: its rows share memory")
+        increment_version(t)  # autograd sees that the tensor is written
+
     def _same(self, batch: KVBatch):
-        if batch.table.device != self.k.device:
-            raise nat.NativeError(f"PagedKVCache: the batch is on {batch.table.device}, the pages on {self.k.device}")
+        if batch._table.device != self._k.device:
+            raise nat.NativeError(f"PagedKVCache: the batch is on {batch._table.device}, the pages on {self._k.device}")
 
     def write(self, k: torch.Tensor, v: torch.Tensor, batch: KVBatch):
         """The batch's new keys and values (rows, heads, 64), fp32, bf16 or fp16, into their pages.  Rows behind the
-        last sequence are not read.  Pages that two sequences share must lie before what is written."""
-        heads = self.k.shape[1]
+        last sequence are not read.  Pages that two sequences share, or that stand twice in one sequence's table, must lie
+        before what is written (two tokens would take one place, in no order)."""
+        heads = self._k.shape[1]
         self._rows(k, "k", heads)
         self._rows(v, "v", heads)
         self._same(batch)
         if k.dtype != v.dtype or k.shape[0] != v.shape[0]:
             raise nat.NativeError("PagedKVCache: k and v must have the same rows and dtype")
-        with nat.on_device(self.k.device):
+        with nat.on_device(self._k.device):
             nat.kv_cache_write(self.desc, batch._rows(k.shape[0]), k, v)
 
     def read(self, batch: KVBatch, cu_rows: torch.Tensor, rows: int, dtype: torch.dtype = torch.bfloat16, out=None):
@@ -147,19 +168,19 @@ class PagedKVCache:
         1, positions past kv_lens[b] as zeros; rows behind the last sequence stay as they are in `out`."""
         self._same(batch)
         _int32(cu_rows, "PagedKVCache: cu_rows", 1)
-        if cu_rows.shape[0] != batch.cu_new.shape[0] or cu_rows.device != self.k.device:
+        if cu_rows.shape[0] != batch._cu_new.shape[0] or cu_rows.device != self._k.device:
             raise nat.NativeError(f"PagedKVCache: cu_rows {tuple(cu_rows.shape)} does not fit the batch")
-        heads = self.k.shape[1]
+        heads = self._k.shape[1]
         if out is None:
             shape = (rows, heads, HEAD_DIM)
-            k, v = self.k.new_empty(shape, dtype=dtype), self.k.new_empty(shape, dtype=dtype)
+            k, v = self._k.new_empty(shape, dtype=dtype), self._k.new_empty(shape, dtype=dtype)
         else:
             k, v = out
             for t, name in ((k, "k"), (v, "v")):
-                self._rows(t, name, heads)
+                self._out(t, name, heads)
                 if t.shape[0] != rows or t.dtype != k.dtype:
                     raise nat.NativeError(f"PagedKVCache: out must hold {rows} rows of one dtype")
-        with nat.on_device(self.k.device):
+        with nat.on_device(self._k.device):
             nat.kv_cache_read(self.desc, batch.desc, cu_rows, rows, k, v)
         return k, v
 
@@ -169,18 +190,18 @@ class PagedKVCache:
         which hold the new tokens' keys and values already.  Query heads are a multiple of the cache's heads (query
         head h reads head h // (query heads // heads)).  mask_block: 0, a token sees its whole sequence; n, it sees up
         to the end of its block of n positions (1: causal; tokens per view: each view itself and the earlier ones).
-        scale: 1/8 by default (None or 0).  No gradient passes.  A token that sees nothing gets zeros and an lse of -inf; rows behind the last sequence
-        are left as they are.  return_lse: also (query heads, rows) fp32 log-sum-exp, as `_native.attn_merge` takes it.
-        """
+        scale: 1/8 by default (None or 0).  out may be q itself, otherwise it must not overlap it.  No gradient passes.
+        A token that sees nothing gets zeros and an lse of -inf; rows behind the last sequence are left as they are.
+        return_lse: also (query heads, rows) fp32 log-sum-exp, as `_native.attn_merge` takes it."""
         self._rows(q, "q")
         self._same(batch)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
-            self._rows(out, "out", q.shape[1])
+            self._out(out, "out", q.shape[1])
             if out.shape[0] != q.shape[0] or out.dtype != q.dtype:
                 raise nat.NativeError("PagedKVCache: out must have q's shape and dtype")
         lse = q.new_empty(q.shape[1], q.shape[0], dtype=torch.float32) if return_lse else None
-        with nat.on_device(self.k.device):
+        with nat.on_device(self._k.device):
             nat.attention_paged(self.desc, batch._rows(q.shape[0]), q, out, lse=lse, scale=scale, mask_block=mask_block)
         return (out, lse) if return_lse else out

@@ -81,8 +81,8 @@ class RoPEAxes:
 
     tokens / keys: (B, H, N, D) fp32, bf16 or fp16 with a contiguous head dim and any other strides (a view of packed
     qkv rows), the head counts of the two may differ.  positions: (B, N, axes) or (N, axes), integer or fp32; angles are
-    formed in 64 bits.  Returns new tensors, or with inplace=True (not for tensors that need a gradient) the rotated
-    inputs, as RoPE2D does."""
+    formed in 64 bits.  Returns new tensors, or with inplace=True (not for tensors that need a gradient, nor for two
+    that share elements) the rotated inputs, as RoPE2D does."""
 
     _LAYOUTS = {"axial": nat.ROPE_AXIAL, "half": nat.ROPE_HALF, "interleaved": nat.ROPE_INTERLEAVED}
 
@@ -143,6 +143,11 @@ class RoPEAxes:
             for t in (tokens, keys):
                 if t is not None and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
                     raise ValueError("RoPEAxes: inplace rotation of an expanded tensor")
+            if keys is not None and keys.numel() and keys.data_ptr() == tokens.data_ptr():
+                raise ValueError("RoPEAxes: inplace rotation of one tensor as tokens and keys")
+            for t in (tokens, keys):
+                if t is not None:
+                    torch.autograd.graph.increment_version(t)  # autograd sees that the tensor is written
             self._run(tokens, keys, positions, False, tokens, keys)
             return tokens if keys is None else (tokens, keys)
         if needs:

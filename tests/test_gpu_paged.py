@@ -565,6 +565,41 @@ def test_paged_class_refusals(nat):
         s.cache.read(s.batch, _ints([0]), 1)
 
 
+@pytest.mark.parametrize("seqs,heads", [([(1, 300)], 4), ([(1, 300), (70, 1300)], 12), ([(300, 2000)], 2)])
+def test_attention_paged_over_its_queries(nat, seqs, heads):
+    """out may be q itself, with one key range and with several."""
+    s = Scene(seqs, 2, 16, torch.bfloat16)
+    s.fill(43)
+    q = _randn(sum(n for n, _ in seqs), heads, 64, seed=41, dtype=torch.bfloat16)
+    want = s.cache.attend(q, s.batch, mask_block=1)
+    mine = q.clone()
+    assert s.cache.attend(mine, s.batch, mask_block=1, out=mine) is mine
+    assert torch.equal(mine, want)
+
+
+def test_paged_outputs_are_seen_and_tensors_are_kept(nat):
+    s = Scene([(2, 40)], 2, 16, torch.bfloat16)
+    q = _randn(2, 4, 64, seed=42, dtype=torch.bfloat16)
+    with pytest.raises(nat.NativeError):
+        s.cache.attend(q, s.batch, out=q[:1].expand(2, 4, 64))
+    with pytest.raises(nat.NativeError):
+        s.cache.attend(q, s.batch, out=q[:, :1].expand(2, 4, 64))
+    cu, k = _ints([0, 40]), torch.zeros(40, 2, 64, device="cuda")
+    with pytest.raises(nat.NativeError):
+        s.cache.read(s.batch, cu, 40, out=(k, k[:1].expand(40, 2, 64)))
+    w = torch.ones((), device="cuda", requires_grad=True)
+    for out, call in ((q, lambda: s.cache.attend(q, s.batch, out=q)),
+                      (k, lambda: s.cache.read(s.batch, cu, 40, out=(k, torch.empty_like(k))))):
+        y = w * out
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+    for t, names in ((s.cache, ("k", "v", "k_exp", "v_exp")), (s.batch, ("table", "kv_lens", "cu_new", "max_new", "max_kv"))):
+        for name in names:  # the calls go by what they were made with
+            with pytest.raises(AttributeError):
+                setattr(t, name, getattr(t, name))
+
+
 # --------------------------------------------------------------------------------------------- together
 @pytest.mark.parametrize("pages", [torch.bfloat16, E4M3, torch.int8], ids=str)
 def test_streaming_run(nat, pages):

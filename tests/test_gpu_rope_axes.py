@@ -203,3 +203,46 @@ def test_rope_axes_empty_and_refused(RoPEAxes):
         r(x.double(), pos)
     with pytest.raises(nat.NativeError):
         r(x.cpu(), pos.cpu())
+
+
+def test_rope_axes_inplace_twice_refused_and_seen_by_autograd(RoPEAxes):
+    r = RoPEAxes((8, 12, 12), freq=100.0)
+    x = torch.randn(1, 2, 4, 64, device="cuda")
+    pos = torch.ones(1, 4, 3, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError):
+        r(x, pos, x, inplace=True)
+    assert all(torch.equal(t, r(x, pos)) for t in r(x, pos, x))
+    w = torch.ones((), device="cuda", requires_grad=True)
+    y = w * x  # keeps x for w's gradient
+    r(x, pos, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_rope_axes_gradient_in_a_graph(RoPEAxes):
+    """Forward and backward captured, replayed with other inputs between eager work; no eager graph of the captured
+    leaf lives meanwhile (torch cannot capture a backward pass then)."""
+    r = RoPEAxes((8, 12, 12), freq=100.0)
+    pos = _positions(2, 70, 3, 500, 51)
+    leaf = _data(2, 3, 70, 64, torch.bfloat16, 50).requires_grad_()
+    up = _data(2, 3, 70, 64, torch.bfloat16, 52)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(r(leaf, pos), leaf, up)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = r(leaf, pos)
+        (grad,) = torch.autograd.grad(out, leaf, up)
+    for i in range(3):
+        with torch.no_grad():
+            leaf.copy_(_data(2, 3, 70, 64, torch.bfloat16, 60 + i))
+            up.copy_(_data(2, 3, 70, 64, torch.bfloat16, 70 + i))
+            pos.add_(5)
+        graph.replay()
+        x = leaf.detach().clone().requires_grad_()
+        y = r(x, pos)
+        (g,) = torch.autograd.grad(y, x, up)
+        torch.cuda.synchronize()
+        assert torch.equal(out, y) and torch.equal(grad, g)

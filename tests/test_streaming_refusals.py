@@ -53,6 +53,15 @@ def test_rope_axes_refuses(nat, over, word):
     assert word in L.mapa_last_error(), L.mapa_last_error()
 
 
+def test_rope_axes_refuses_one_output_for_both(nat):
+    L = nat.load_library()
+    assert L.mapa_rope_axes(ctypes.byref(_rope(nat, x=(4096, 4096), y=(4096, 4096), heads=(2, 2),
+                                               **{k: (s, s) for k, s in (("x_bstride", 512), ("y_bstride", 512),
+                                                  ("x_hstride", 64), ("y_hstride", 64), ("x_nstride", 128),
+                                                  ("y_nstride", 128))})), None) != 0
+    assert b"one output" in L.mapa_last_error()
+
+
 def test_rope_axes_nothing_to_do(nat):
     L = nat.load_library()
     assert L.mapa_rope_axes(None, None) != 0
