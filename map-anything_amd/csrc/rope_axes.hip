@@ -169,8 +169,12 @@ __global__ void __launch_bounds__(TPB) rope_axes_kernel(RopeArgs a) {
           T& ur = PAIRED ? lo[k].e[PAIRED ? 2 * j : j] : lo[k].e[j];
           T& vr = PAIRED ? lo[k].e[PAIRED ? 2 * j + 1 : j] : hi[k].e[j];
           const float u = to_f32<DT>(ur), v = to_f32<DT>(vr);
-          ur = from_f32<DT>(u * c - v * s);
-          vr = from_f32<DT>(v * c + u * s);
+          float nu = __builtin_fmaf(u, c, -(v * s)), nv = __builtin_fmaf(v, c, u * s);
+          // fp32 first in every variant: some took an fma that rounds to fp16 at once, so that fp16 results differed by
+          // alignment
+          if constexpr (DT == MAPA_F16) asm("" : "+v"(nu), "+v"(nv));
+          ur = from_f32<DT>(nu);
+          vr = from_f32<DT>(nv);
         }
         if constexpr (PAIRED && W == 1) {
           out[k][0] = lo[k].e[0];

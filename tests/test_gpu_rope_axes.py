@@ -246,3 +246,20 @@ def test_rope_axes_gradient_in_a_graph(RoPEAxes):
         (g,) = torch.autograd.grad(y, x, up)
         torch.cuda.synchronize()
         assert torch.equal(out, y) and torch.equal(grad, g)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("layout", ["axial", "half", "interleaved"])
+@pytest.mark.parametrize("sections,D", [((32,), 64), ((16, 2, 2, 8), 56), ((8, 4), 26), ((2,), 4)])
+def test_rope_axes_alignment_does_not_change_results(RoPEAxes, dtype, layout, sections, D):
+    """Bit for bit the same from aligned rows, from rows one value further and in place in rows of odd length."""
+    r = RoPEAxes(sections, freq=100.0, layout=layout)
+    x = _data(2, 3, 1500, D, dtype, 80)
+    pos = _positions(2, 1500, len(sections), 50, 81)
+    want = r(x, pos)
+    odd = torch.zeros(2, 3, 1500, D + 9, dtype=dtype, device="cuda")
+    odd[..., 1: D + 1] = x
+    assert torch.equal(r(odd[..., 1: D + 1], pos), want)
+    r(odd[..., 1: D + 1], pos, inplace=True)
+    assert torch.equal(odd[..., 1: D + 1], want)
+    assert (odd[..., 0] == 0).all() and (odd[..., D + 1:] == 0).all()
