@@ -1156,9 +1156,9 @@ int ragged_splits(int64_t tasks, int tiles, int slots, double fixed, int most) {
 }
 
 // Waves of a chunk workgroup (32 rows each).  Eight share a tile's decoding where two workgroups of four do it twice: an
-// 8-view chunk over int8 pages takes 779 us with eight and 860 with four (e4m3 739 and 765), a 1370-token view over 100
-// views 737 and 793 (702 and 713) though a twelfth of its eight-wave rows is empty.  16-bit pages have nothing to decode
-// (695 and 701 us, 676 and 670), and ragged batches want the finer pieces (ragged causal int8 chunks 134 and 121 us).
+// 8-view chunk over int8 pages takes 729 us with eight and 785 with four (e4m3 691 and 706), a 1370-token view over 100
+// views 717 and 767 (680 and 693) though a twelfth of its eight-wave rows is empty.  16-bit pages have nothing to decode
+// (642 and 633 us, 656 and 659), and ragged batches want the finer pieces (ragged causal int8 chunks 133 and 122 us).
 int chunk_waves(const mapa_attn_paged_desc& d) {
   const bool codes = d.cache.dtype == MAPA_FP8 || d.cache.dtype == MAPA_I8;
   const int64_t rows = (int64_t)d.batch.max_new * (d.heads / d.cache.heads);
