@@ -30,6 +30,7 @@ from __future__ import annotations
 
 import json
 import os
+import threading
 import warnings
 from collections import OrderedDict
 from typing import Any, Dict, List, Optional
@@ -83,6 +84,27 @@ def _check_config(encoder_config, info_sharing_config, pred_head_config):
     if problems:
         raise ValueError("MapAnything (MI355X engine) implements the released architecture "
                          f"(configs/inference.json); unsupported: {', '.join(problems)}")
+
+
+class _ForwardGraph(torch.cuda.CUDAGraph):
+    """The graph of a forward, registered with a random-generator state of its own.  torch registers every graph with the
+    device's default generator, and the first one alive makes the two tensors that all later captures write: under
+    inference mode, where the forwards are captured, these would be inference tensors, and a caller's capture outside
+    inference mode would raise for as long as one of the model's graphs lives.  A forward draws no random numbers, so
+    its capture begins on a copy of the state; the default generator itself stays as it is (the copy stands in for it
+    during that one call)."""
+
+    _swap = threading.Lock()  # rank threads of a sharded model capture at once
+
+    def capture_begin(self, *args, **kwargs):
+        gen = torch.cuda.default_generators[torch.cuda.current_device()]
+        with self._swap:
+            own = gen.graphsafe_get_state()
+            gen.graphsafe_set_state(gen.clone_state())
+            try:
+                super().capture_begin(*args, **kwargs)
+            finally:
+                gen.graphsafe_set_state(own)
 
 
 class MapAnything:
@@ -589,7 +611,7 @@ class MapAnything:
                         if not (e.range_only and eng.hsplit and eng.hfmt in ("f16", "f16x2")):
                             raise
                 torch.cuda.current_stream(imgs.device).wait_stream(side)
-                graph = torch.cuda.CUDAGraph()
+                graph = _ForwardGraph()
                 gslot = nat.FaultSlot()  # the graph's own publish slot (its address is baked into the graph)
                 # captured on the warm-up stream: the per-stream GEMM / attention workspaces made in the warm-up
                 # are the ones the graph uses (no allocation or zero-fill inside the capture).  With a shard the
