@@ -155,6 +155,14 @@ __device__ __forceinline__ bf16x8 only(bf16x8 v, int j) {
   return __builtin_bit_cast(bf16x8, r);
 }
 
+// A row's sum l over the keys it sees, at the reference m (log2 domain), is positive unless all their scores are -inf.
+// The whole row is 0 / 0 = NaN then; a range of it (part) leaves zeros and a logarithm of -inf, which weigh nothing beside
+// the other ranges.
+__device__ __forceinline__ float range_inverse(float l, bool part) { return part && l == 0.f ? 1.f : 1.f / l; }
+__device__ __forceinline__ float range_lse(float m, float l, bool part) {
+  return l > 0.f ? m + __log2f(l) : part && l == 0.f ? -INFINITY : __builtin_nanf("");
+}
+
 // Row tile of the chunk kernel -> (sequence, its first packed row, its new and its cached tokens, tile in it), by a
 // wave-wide prefix sum over the sequences' tile counts, 64 at a time; seq -1: no such tile.
 struct RowTile {
@@ -622,10 +630,10 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_paged_chunk(PagedArgs p) {
   pv_checked(lds + (2 + ((kt1 - 1 - kt0) & 1)) * TILE, kt1 - 1);
 
   const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
-  // a row that sees keys of the range has a sum of one at least, unless every score is -inf (then NaN, as the formula)
   const bool seen = limit > k_begin;
-  const float inv = seen ? 1.f / l_tot : 0.f;
-  const float lse2 = !seen ? -INFINITY : l_tot > 0.f ? m_ref + __log2f(l_tot) : __builtin_nanf("");
+  const bool part = slot >= 0;
+  const float inv = !seen ? 0.f : range_inverse(l_tot, part);
+  const float lse2 = !seen ? -INFINITY : range_lse(m_ref, l_tot, part);
   if (!seen) {
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt)
@@ -953,11 +961,11 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
       l += wgt * join_l[x][row];
       acc += wgt * *reinterpret_cast<const f32x4*>(jo + (x * RS + row) * HD + d);
     }
-    const float inv = 1.f / l;
-    const float lse2 = !seen ? -INFINITY : l > 0.f ? m_use + __log2f(l) : __builtin_nanf("");
-    f32x4 v = acc * inv;
+    const bool part = lim_hi > p.chunk;
+    const float lse2 = !seen ? -INFINITY : range_lse(m_use, l, part);
+    f32x4 v = acc * range_inverse(l, part);
     if (!seen) v = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (lim_hi <= p.chunk) {  // one range holds all keys: no partials
+    if (!part) {  // one range holds all keys: no partials
       *reinterpret_cast<uint2*>(p.o + (int64_t)t * p.orr + h * p.oh + d) =
           uint2{pack16<F16>(v[0], v[1]), pack16<F16>(v[2], v[3])};
       if (p.lse && d == 0) p.lse[(int64_t)h * p.new_rows + t] = lse2 * LN2;
@@ -994,7 +1002,7 @@ __device__ __forceinline__ void merge_store(const PagedArgs& p, int n, float m, 
   *reinterpret_cast<uint2*>(p.o + (int64_t)tok * p.orr + head * p.oh + d) =
       uint2{pack16<F16>(acc[0] * inv, acc[1] * inv), pack16<F16>(acc[2] * inv, acc[3] * inv)};
   if (p.lse && d == 0)
-    p.lse[(int64_t)head * p.new_rows + tok] = n > 0 ? ((m == -INFINITY ? 0.f : m) + __log2f(l)) * LN2 : -INFINITY;
+    p.lse[(int64_t)head * p.new_rows + tok] = n > 0 ? range_lse(m, l, false) * LN2 : -INFINITY;
 }
 
 // One wave per row: four groups of 16 lanes x 4 columns, group g over the key ranges g, g + 4, ...; 32 ranges' partials
