@@ -133,18 +133,28 @@ __device__ __forceinline__ bf16x8 decode8(uint2 w, float s) {
   }
 }
 
-// whether any of 8 operand words is an infinity or a NaN
+// Bits 15 and 31 of the result: whether any of 8 operand words is an infinity or a NaN (an exponent of all ones carries)
 template <bool F16>
-__device__ __forceinline__ bool any_special(bf16x8 v) {
-  constexpr uint32_t E = F16 ? 0x7c007c00u : 0x7f807f80u, LO = E & 0xffffu, HI = E & 0xffff0000u;
+__device__ __forceinline__ uint32_t special_bits(uint32_t w) {
+  constexpr uint32_t E = F16 ? 0x7c007c00u : 0x7f807f80u, ONE = F16 ? 0x04000400u : 0x00800080u;
+  return ((w & E) + ONE) & 0x80008000u;
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t special_bits(bf16x8 v) {
   const uint4 u = __builtin_bit_cast(uint4, v);
-  bool r = false;
+  return special_bits<F16>(u.x) | special_bits<F16>(u.y) | special_bits<F16>(u.z) | special_bits<F16>(u.w);
+}
+// 8 operand words with zeros for the infinities and NaNs (SPECIAL: for all others)
+template <bool F16, bool SPECIAL>
+__device__ __forceinline__ bf16x8 part_of(bf16x8 v) {
+  const uint4 u = __builtin_bit_cast(uint4, v);
+  uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t w = i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w;
-    r |= ((w & LO) == LO) | ((w & HI) == HI);
+    const uint32_t b = special_bits<F16>(w[i]), m = (b - (b >> 15)) | b;  // 16 ones for each
+    w[i] &= SPECIAL ? m : ~m;
   }
-  return r;
+  return __builtin_bit_cast(bf16x8, uint4{w[0], w[1], w[2], w[3]});
 }
 // element j of 8 operand words, the others zero
 __device__ __forceinline__ bf16x8 only(bf16x8 v, int j) {
@@ -449,42 +459,48 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_paged_chunk(PagedArgs p) {
       }
   };
   // O^T += V^T P^T of tile kt, with a look at V first: an infinity or NaN of a key that some rows do not see, times
-  // their zero probability, must not reach them — such a tile is added key by key, where it is seen
+  // their zero probability, must not reach them.  The product takes zeros in their place (so that a row's sum is formed
+  // the same way whatever its hidden keys hold), and they are added key by key, where they are seen.
   auto pv_checked = [&](const char* Vs, int kt) __attribute__((always_inline)) {
     bf16x8 vf[2][4];
-    bool special = false;
+    uint32_t bits = 0;
 #pragma unroll
     for (int f = 0; f < 4; ++f)
 #pragma unroll
       for (int dt = 0; dt < 2; ++dt) {
         vf[dt][f] = v_frag(Vs, dt, f);
-        special |= any_special<F16>(vf[dt][f]);
+        bits |= special_bits<F16>(vf[dt][f]);
       }
-    if (__builtin_expect(__any(special), 0)) {
+    const bool special = __any(bits != 0);
+    if (__builtin_expect(special, 0)) {
 #pragma unroll
       for (int f = 0; f < 4; ++f)
+#pragma unroll
+        for (int dt = 0; dt < 2; ++dt) vf[dt][f] = part_of<F16, false>(vf[dt][f]);
+    }
+#pragma unroll
+    for (int f = 0; f < 4; ++f)
+#pragma unroll
+      for (int dt = 0; dt < 2; ++dt) o[dt] = mfma32x32x16<F16>(vf[dt][f], pf[f], o[dt]);
+    if (__builtin_expect(special, 0)) {
+      asm volatile("" ::: "memory");  // the fragments are read again: kept over the product, they would spill
+      const bf16x8 p0 = pf[0], p1 = pf[1], p2 = pf[2], p3 = pf[3];
+#pragma unroll
+      for (int dt = 0; dt < 2; ++dt)
 #pragma unroll 1
-        for (int jj = 0; jj < 16; ++jj) {
-          const int j = jj & 7, h2 = jj >> 3;
+        for (int fj = 0; fj < 64; ++fj) {
+          const int f = fj >> 4, j = fj & 7, h2 = (fj >> 3) & 1;
           const int key = kt * KT + 16 * f + (j & 3) + 8 * (j >> 2) + 4 * h2;
           const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
-          const bf16x8 pk = hl == h2 ? only(pf[f], j) : z;
+          const bf16x8 pr = f == 0 ? p0 : f == 1 ? p1 : f == 2 ? p2 : p3;
+          const bf16x8 pk = hl == h2 ? only(pr, j) : z, vk = hl == h2 ? only(part_of<F16, true>(v_frag(Vs, dt, f)), j) : z;
+          f32x16 t;
 #pragma unroll
-          for (int dt = 0; dt < 2; ++dt) {
-            const bf16x8 vk = hl == h2 ? only(vf[dt][f], j) : z;
-            f32x16 t;
+          for (int i = 0; i < 16; ++i) t[i] = 0.f;
+          t = mfma32x32x16<F16>(vk, pk, t);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) t[i] = 0.f;
-            t = mfma32x32x16<F16>(vk, pk, t);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[dt][i] = key < limit ? o[dt][i] + t[i] : o[dt][i];
-          }
+          for (int i = 0; i < 16; ++i) o[dt][i] = key < limit ? o[dt][i] + t[i] : o[dt][i];
         }
-    } else {
-#pragma unroll
-      for (int f = 0; f < 4; ++f)
-#pragma unroll
-        for (int dt = 0; dt < 2; ++dt) o[dt] = mfma32x32x16<F16>(vf[dt][f], pf[f], o[dt]);
     }
   };
 
@@ -574,8 +590,14 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_paged_chunk(PagedArgs p) {
     }
     float ls = (a[0] + a[1]) + (a[2] + a[3]);
     if constexpr (!FIRST) {
-      if (__builtin_expect(__any(!(ls <= REBASE_SUM)), 0)) {  // NaN rebases too
-        const float m = fmaxf(row_max(s), m_ref);
+      const uint64_t over = __ballot(!(ls <= REBASE_SUM));  // NaN rebases too
+      if (__builtin_expect(over != 0, 0)) {
+        // a row (its two lanes) moves its reference by its own scores: the wave's other rows compute what they have again.
+        // The maximum exchanges values between lanes, so all of them take part in it (kept out of a branch by the asm).
+        const bool mine = ((over | over << 32 | over >> 32) >> lane) & 1;
+        float m = fmaxf(row_max(s), m_ref);
+        asm volatile("" : "+v"(m));
+        m = mine ? m : m_ref;
         const float alpha = __builtin_amdgcn_exp2f(m_ref - m);
         m_ref = m;
         l_run *= alpha;
@@ -583,7 +605,7 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_paged_chunk(PagedArgs p) {
         for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
           for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
-        ls = 0.f;
+        float again = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           uint32_t pk[4];
@@ -592,11 +614,13 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_paged_chunk(PagedArgs p) {
             const int e = 8 * (i & 1) + 2 * g;
             const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 1][e], c, -m));
             const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 1][e + 1], c, -m));
-            ls += e0 + e1;
+            again += e0 + e1;
             pk[g] = pack16<F16>(e0, e1);
           }
           pf[i] = __builtin_bit_cast(bf16x8, uint4{pk[0], pk[1], pk[2], pk[3]});
         }
+        asm volatile("" : "+v"(again));
+        ls = mine ? again : ls;
       }
     }
     l_run += ls;
@@ -612,6 +636,9 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_paged_chunk(PagedArgs p) {
     for (int kk = 0; kk < 4; ++kk) st[0][kb] = mfma32x32x16<F16>(k_frag(lds, kb, kk), qf[kk], st[0][kb]);
   }
   step_barrier();  // K of the first tile is read: its slot is free
+  // Nothing is in flight here.  The compiler does not see that in the asm above: without its own wait it may put one for
+  // Q's loads into the loop, where it waits for the step's DMA (5 % of a view over a 100-view scene)
+  if constexpr (CK == 0) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   int kt = kt0;
   if (kt < kt_free) step(kt, T_(), F_(), P0());
   else step(kt, T_(), T_(), P0());
@@ -845,20 +872,26 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
       }
     }
     // V^T fragments: dims 16 dt + l16, keys 4 g .. + 3 and 16 + 4 g .. + 3 (the order the scores come in)
-    bf16x8 vf[4];
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt) {
+    auto v_frag = [&](int dt) __attribute__((always_inline)) {
       const int q4 = l16 >> 2, p4 = l16 & 3;
       const int row = 4 * g + q4, ch = dt * 2 + (p4 >> 1), within = (p4 & 1) * 8;
       const s4v lo = tr_read(vslot(row, ch) + within);
       const s4v hi = tr_read(vslot(row + 16, ch) + within);
-      vf[dt] = s8v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    }
-    bool special = false;
-    if (mask) {
+      return (bf16x8)s8v{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
+    bf16x8 vf[4];
 #pragma unroll
-      for (int dt = 0; dt < 4; ++dt) special |= any_special<F16>(vf[dt]);
-      special = __any(special);
+    for (int dt = 0; dt < 4; ++dt) vf[dt] = v_frag(dt);
+    bool special = false;  // as in the chunk kernel's pv_checked
+    if (mask) {
+      uint32_t bits = 0;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) bits |= special_bits<F16>(vf[dt]);
+      special = __any(bits != 0);
+    }
+    if (__builtin_expect(special, 0)) {
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) vf[dt] = part_of<F16, false>(vf[dt]);
     }
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
@@ -893,24 +926,28 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
                                                          pack16<F16>(e[4], e[5]), pack16<F16>(e[6], e[7])});
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt) o[rb][dt] *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) o[rb][dt] = mfma16x16x32<F16>(vf[dt], pf, o[rb][dt]);
       if (__builtin_expect(special, 0)) {
 #pragma unroll 1
-        for (int jj = 0; jj < 32; ++jj) {  // one key at a time, added where it is seen
-          const int j = jj & 7, g2 = jj >> 3;
-          const int key = key0 + 4 * g2 + (j & 3) + 16 * (j >> 2);
-          const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
-          const bf16x8 pk = g == g2 ? only(pf, j) : z;
+        for (int dt = 0; dt < 4; ++dt) {
+          const bf16x8 vs = part_of<F16, true>(v_frag(dt));
+          f32x4 sum = o[rb][0];
 #pragma unroll
-          for (int dt = 0; dt < 4; ++dt) {
-            const bf16x8 vk = g == g2 ? only(vf[dt], j) : z;
+          for (int x = 1; x < 4; ++x) sum = dt == x ? o[rb][x] : sum;
+#pragma unroll 1
+          for (int jj = 0; jj < 32; ++jj) {
+            const int j = jj & 7, g2 = jj >> 3;
+            const int key = key0 + 4 * g2 + (j & 3) + 16 * (j >> 2);
+            const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+            const bf16x8 pk = g == g2 ? only(pf, j) : z, vk = g == g2 ? only(vs, j) : z;
             const f32x4 x = mfma16x16x32<F16>(vk, pk, f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[rb][dt][i] = key < limit[rb] ? o[rb][dt][i] + x[i] : o[rb][dt][i];
+            for (int i = 0; i < 4; ++i) sum[i] = key < limit[rb] ? sum[i] + x[i] : sum[i];
           }
-        }
-      } else {
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt) o[rb][dt] = mfma16x16x32<F16>(vf[dt], pf, o[rb][dt]);
+          for (int x = 0; x < 4; ++x) o[rb][x] = dt == x ? sum : o[rb][x];
+        }
       }
     }
   };

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import streaming_ref as ref
-from test_gpu_paged import Scene, _randn, nat, no_fault  # noqa: F401  (fixtures)
+from test_gpu_paged import E4M3, Scene, _randn, nat, no_fault  # noqa: F401  (fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -58,3 +58,53 @@ def test_ranges_of_minus_infinity(nat, kind, split, dead, shape):
     wlse[:, none] = math.nan
     ref.within(got, want, tol, "out")
     ref.within(lse, wlse, ltol, "lse")
+
+
+@pytest.mark.parametrize("kind,pages", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16),
+                                        (torch.bfloat16, E4M3), (torch.float16, torch.int8)], ids=str)
+@pytest.mark.parametrize("seqs,heads,kv_heads", [([(6, 70), (3, 3)], 4, 2), ([(100, 260), (40, 40)], 4, 2),
+                                                 ([(300, 900)], 2, 2), ([(500, 3000)], 2, 1)])
+@pytest.mark.parametrize("block", [1, 5])
+@pytest.mark.parametrize("split", [True, False])
+def test_results_do_not_depend_on_what_is_hidden(nat, kind, pages, seqs, heads, kv_heads, block, split):
+    """Bit for bit the same for the rows that do not see a token, whatever its key and value are: a score that moves its
+    neighbours' reference, a NaN, an infinite value.  The first keys' scores are small, so that the rows' references lie
+    below what follows and a step that moved them all would show."""
+    at = [0]
+    for _, t in seqs:
+        at.append(at[-1] + t)
+    which = [t - 1 - min(n // 2, 20) for n, t in seqs]  # the token of each sequence that changes
+
+    def run(change):
+        def spoil(batch, k, v):
+            k *= 0.4
+            for a, i in zip(at, which):
+                k[a: a + min(64, i)] *= 0.1
+                if change:
+                    change(k, v, a + i)
+
+        s = Scene(seqs, kv_heads, 16, pages)
+        s.fill(21, kind, change=spoil)
+        return _attend(nat, s, q, block, split)
+
+    q = _randn(sum(n for n, _ in seqs), heads, 64, seed=2, dtype=kind)
+    hidden = torch.cat([torch.tensor([x <= i for x in ref.limits(n, t, block)]) for (n, t), i in zip(seqs, which)]).cuda()
+    assert hidden.any()
+    want, wlse = run(None)
+
+    def large(k, v, i):  # the rows that see it move their reference by dozens
+        k[i] *= 150
+
+    def nan_key(k, v, i):
+        k[i, :, 7] = math.nan
+
+    def infinite(k, v, i):
+        v[i, :, 5] = math.inf
+        v[i, :, 9] = math.nan
+
+    for change in (large, nan_key, infinite):
+        got, lse = run(change)
+        assert torch.equal(got[hidden], want[hidden]), change.__name__
+        assert torch.equal(lse[:, hidden], wlse[:, hidden]), change.__name__
+        if change is large:
+            assert not torch.equal(got[~hidden], want[~hidden])
