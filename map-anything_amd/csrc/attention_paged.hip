@@ -6,7 +6,8 @@
 // Rows are (new token, query head of the group) pairs, token-major, so that all query heads of a K/V head share its
 // tiles.  Q enters the MFMA as it is and c is applied to the fp32 scores: folding c into a 16-bit Q would round it once
 // more, which costs as much accuracy as the rounding of the output.  P is rounded to 16 bits as an MFMA operand, its
-// sum is not.  The sums' reference m_i is the row's first tile's maximum, moved only when a tile's sum passes 2^8.
+// sum is not.  The sums' reference m_i is the row's first tile's maximum (2^7 below it in fp16), moved only when a
+// tile's sum passes 2^8 (2^15).
 //
 //  * attn_paged_chunk: 4 or 8 waves x 32 rows over 64-key tiles (as mapa_attention): S^T = K Q^T on 32x32x16 MFMAs, so
 //    a lane owns a row and P feeds O^T = V^T P^T without leaving registers.  16-bit pages go to LDS by DMA, 8-bit pages
@@ -36,7 +37,14 @@ constexpr int KT = 64;   // keys of a chunk tile
 constexpr int ST = 32;   // keys of a step tile
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
-constexpr float REBASE_SUM = 256.f;
+// A row's reference moves when a tile's sum of probabilities passes REBASE_SUM.  In fp16 the reference lies LIFT below the
+// row's first maximum and probabilities go up to 2^15: fp16's smallest steps then lose 2^-32 of the row's largest at
+// most, not 2^-25.  20 thousand keys 18 below a single one, which weigh 3e-4 together, came out as nothing without it.
+template <bool F16>
+struct Softmax {
+  static constexpr float LIFT = F16 ? 7.f : 0.f;  // log2
+  static constexpr float REBASE_SUM = F16 ? 32768.f : 256.f;
+};
 
 struct PagedArgs {
   const char* page[2];  // K, V
@@ -544,7 +552,8 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_paged_chunk(PagedArgs p) {
       }
     }
     if constexpr (MASK) hide(s, t);
-    if constexpr (FIRST) m_ref = fmaxf(row_max(s), -1e38f);  // finite also for a row that sees none of the range
+    // finite also for a row that sees none of the range
+    if constexpr (FIRST) m_ref = fmaxf(row_max(s), -1e38f) - Softmax<F16>::LIFT;
     const float nm = -m_ref;
     if constexpr (MASK && !FIRST) pv_checked(Vs, t - 1);
     // Group n: MFMA n; the exponents of scores 2n, 2n + 1; behind them the sums and the conversion of the two before,
@@ -590,12 +599,12 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_paged_chunk(PagedArgs p) {
     }
     float ls = (a[0] + a[1]) + (a[2] + a[3]);
     if constexpr (!FIRST) {
-      const uint64_t over = __ballot(!(ls <= REBASE_SUM));  // NaN rebases too
+      const uint64_t over = __ballot(!(ls <= Softmax<F16>::REBASE_SUM));  // NaN rebases too
       if (__builtin_expect(over != 0, 0)) {
         // a row (its two lanes) moves its reference by its own scores: the wave's other rows compute what they have again.
         // The maximum exchanges values between lanes, so all of them take part in it (kept out of a branch by the asm).
         const bool mine = ((over | over << 32 | over >> 32) >> lane) & 1;
-        float m = fmaxf(row_max(s), m_ref);
+        float m = fmaxf(row_max(s) - Softmax<F16>::LIFT, m_ref);
         asm volatile("" : "+v"(m));
         m = mine ? m : m_ref;
         const float alpha = __builtin_amdgcn_exp2f(m_ref - m);
@@ -911,7 +920,7 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
                        fmaxf(fmaxf(st[1][0], st[1][1]), fmaxf(st[1][2], st[1][3])));
       mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
       mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
-      const float m_new = fmaxf(m_ref[rb], mx);
+      const float m_new = fmaxf(m_ref[rb], mx - Softmax<F16>::LIFT);
       const float m_use = m_new == -INFINITY ? 0.f : m_new;  // nothing seen yet
       const float alpha = __builtin_amdgcn_exp2f(m_ref[rb] - m_use);
       m_ref[rb] = m_new;

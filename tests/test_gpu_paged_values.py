@@ -60,6 +60,57 @@ def test_ranges_of_minus_infinity(nat, kind, split, dead, shape):
     ref.within(lse, wlse, ltol, "lse")
 
 
+@pytest.mark.parametrize("gap", [12, 14, 16, 17, 18])
+@pytest.mark.parametrize("shape", [([(1, 20000)], 2, 2), ([(3, 20000)], 8, 2), ([(70, 20000)], 2, 2)])
+def test_small_probabilities_in_fp16(nat, gap, shape):
+    """One key `gap` above 20 thousand others, its value 0 and theirs about 1: what the small ones add up to is not lost.
+    P carries a factor of 2^7, so that one under fp16's smallest steps is off by 2^-25 2^-7 of the row's largest at
+    most, n of them against a sum of at least one."""
+    seqs, heads, kv_heads = shape
+    n = seqs[0][1]
+
+    def peak(batch, k, v):
+        k.zero_()
+        k[0, :, 0] = gap
+        v.uniform_(0.5, 1, generator=torch.Generator(device="cuda").manual_seed(1))
+        v[1] = 1
+        v[0] = 0
+
+    s = Scene(seqs, kv_heads, 64, torch.float16)
+    s.fill(1, torch.float16, change=peak)
+    q = torch.zeros(s.rows, heads, 64, dtype=torch.float16, device="cuda")
+    q[:, :, 0] = 8
+    want, wlse, tol, ltol = s.expect(q, 1)
+    tol = tol - n * 2.0 ** -25 + n * 2.0 ** -32
+    for split in (True, False):
+        got, lse = _attend(nat, s, q, 1, split)
+        ref.within(got, want, tol, "out")
+        ref.within(lse, wlse, ltol, "lse")
+
+
+@pytest.mark.parametrize("seqs,heads,kv_heads", [([(1, 5000), (1, 80)], 12, 12), ([(200, 900)], 4, 4), ([(4, 700)], 8, 2)])
+@pytest.mark.parametrize("pages", [torch.float16, torch.int8], ids=str)
+@pytest.mark.parametrize("top", [1, 12, 30])
+def test_growing_scores_in_fp16(nat, seqs, heads, kv_heads, pages, top):
+    """Keys that grow along the sequence, slowly and fast: probabilities pass the reference's again and again and stay
+    within fp16."""
+    s = Scene(seqs, kv_heads, 32, pages)
+
+    def grow(batch, k, v):
+        at = batch.cu_new.tolist()
+        for a, b in zip(at, at[1:]):
+            k[a:b] *= torch.linspace(0.1, top, b - a, device="cuda")[:, None, None].to(k.dtype)
+        v *= 100
+
+    s.fill(3, torch.float16, change=grow)
+    q = _randn(s.rows, heads, 64, seed=9, dtype=torch.float16)
+    for split in (True, False):
+        got, lse = _attend(nat, s, q, 1, split)
+        want, wlse, tol, ltol = s.expect(q, 1)
+        ref.within(got, want, tol, "out")
+        ref.within(lse, wlse, ltol, "lse")
+
+
 @pytest.mark.parametrize("kind,pages", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16),
                                         (torch.bfloat16, E4M3), (torch.float16, torch.int8)], ids=str)
 @pytest.mark.parametrize("seqs,heads,kv_heads", [([(6, 70), (3, 3)], 4, 2), ([(100, 260), (40, 40)], 4, 2),
