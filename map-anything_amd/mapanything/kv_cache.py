@@ -85,7 +85,7 @@ class PagedKVCache:
     code * 2^(byte - 127), see include/mapa.h).  page_size: a power of two, 16 to 1024.  The tensors are the cache's
     for its life: their contents may be moved or filled, larger ones make another cache (wrap)."""
 
-    __slots__ = ("_k", "_v", "_k_exp", "_v_exp", "desc")
+    __slots__ = ("_k", "_v", "_k_exp", "_v_exp", "_tensors", "desc")
 
     k = property(lambda self: self._k)
     v = property(lambda self: self._v)
@@ -124,6 +124,7 @@ class PagedKVCache:
                 if e.dtype != torch.uint8 or e.shape != k.shape[:3] or not e.is_contiguous() or e.device != k.device:
                     raise nat.NativeError("PagedKVCache: exponents must be contiguous uint8 (pages, heads, page_size)")
         self._k, self._v, self._k_exp, self._v_exp = k, v, k_exp, v_exp
+        self._tensors = (k, v) if k_exp is None else (k, v, k_exp, v_exp)
         self.desc = nat.KVCacheDesc(code, k.shape[1], k.shape[2], k.shape[0], k.data_ptr(), v.data_ptr(),
                                     None if k_exp is None else k_exp.data_ptr(),
                                     None if v_exp is None else v_exp.data_ptr())
@@ -160,6 +161,7 @@ class PagedKVCache:
         self._same(batch)
         if k.dtype != v.dtype or k.shape[0] != v.shape[0]:
             raise nat.NativeError("PagedKVCache: k and v must have the same rows and dtype")
+        increment_version(self._tensors)  # autograd sees that they are written
         with nat.on_device(self._k.device):
             nat.kv_cache_write(self.desc, batch._rows(k.shape[0]), k, v)
 

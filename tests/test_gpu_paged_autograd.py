@@ -1,0 +1,30 @@
+"""The paged cache beside autograd."""
+
+import pytest
+import torch
+
+from test_gpu_paged import E4M3, Scene, _randn, nat, no_fault  # noqa: F401  (fixtures)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("pages", [torch.bfloat16, torch.float16, E4M3, torch.int8], ids=str)
+def test_write_is_seen_by_autograd(nat, pages):
+    """A graph that keeps the pages (or their exponents) does not go backward over what a later write left in them."""
+    s = Scene([(2, 40)], 2, 16, pages)
+    s.fill(1)
+    rows = _randn(2, 2, 64, seed=2, dtype=torch.bfloat16)
+    tensors = [t for t in (s.cache.k, s.cache.v, s.cache.k_exp, s.cache.v_exp) if t is not None]
+    before = [t._version for t in tensors]
+    s.cache.write(rows, rows, s.batch)
+    assert all(t._version > b for t, b in zip(tensors, before))
+    if pages == torch.bfloat16:
+        w = torch.ones((), dtype=pages, device="cuda", requires_grad=True)
+        y = (w * s.cache.k[0]).sum()
+        s.cache.write(rows, rows, s.batch)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():  # pages without a version counter of their own
+        t = Scene([(2, 40)], 2, 16, pages)
+        t.cache.write(rows, rows, t.batch)
+        s.cache.write(rows, rows, s.batch)
