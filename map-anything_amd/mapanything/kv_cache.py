@@ -150,6 +150,9 @@ class PagedKVCache:
     def _same(self, batch: KVBatch):
         if batch._table.device != self._k.device:
             raise nat.NativeError(f"PagedKVCache: the batch is on {batch._table.device}, the pages on {self._k.device}")
+        if (self._k.requires_grad or self._v.requires_grad) and torch.is_grad_enabled():
+            raise nat.NativeError("PagedKVCache: the pages need a gradient, and none passes through the cache "
+                                  "(torch.no_grad() or detach())")
 
     def write(self, k: torch.Tensor, v: torch.Tensor, batch: KVBatch):
         """The batch's new keys and values (rows, heads, 64), fp32, bf16 or fp16, into their pages.  Rows behind the

@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from test_gpu_paged import E4M3, Scene, _randn, nat, no_fault  # noqa: F401  (fixtures)
+from test_gpu_paged import E4M3, Scene, _ints, _randn, nat, no_fault  # noqa: F401  (fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -28,3 +28,23 @@ def test_write_is_seen_by_autograd(nat, pages):
         t = Scene([(2, 40)], 2, 16, pages)
         t.cache.write(rows, rows, t.batch)
         s.cache.write(rows, rows, s.batch)
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_pages_that_need_a_gradient_are_refused(nat, which):
+    from mapanything.kv_cache import PagedKVCache
+
+    s = Scene([(2, 40)], 2, 16, torch.bfloat16)
+    s.fill(1)
+    pages = {x: getattr(s.cache, x).detach().clone() for x in ("k", "v")}
+    leaf = pages[which].requires_grad_()
+    rows = _randn(2, 2, 64, seed=2, dtype=torch.bfloat16)
+    cu = _ints([0, 40])
+    for held in (pages, {**pages, which: leaf * 1}):  # a leaf, and what was computed from one
+        cache = PagedKVCache.wrap(held["k"], held["v"])
+        for call in (lambda: cache.attend(rows, s.batch), lambda: cache.read(s.batch, cu, 40),
+                     lambda: cache.write(rows, rows, s.batch)):
+            with pytest.raises(nat.NativeError, match="gradient"):
+                call()
+            with torch.no_grad():
+                call()
