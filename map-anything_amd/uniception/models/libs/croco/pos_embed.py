@@ -49,21 +49,24 @@ class _RoPEAxesTurn(torch.autograd.Function):
     the tangents, and its backward the turn of the gradients the other way."""
 
     @staticmethod
-    def forward(ctx, rope, inverse, positions, tokens, keys):
+    def forward(ctx, rope, inverse, positions, tokens, keys, still=None):  # still: the output that needs no gradient
         ctx.rope, ctx.inverse = rope, inverse
         ctx.shapes = [None if t is None else t.shape for t in (tokens, keys)]
         ctx.save_for_backward(positions)
         ctx.save_for_forward(positions)
         ctx.set_materialize_grads(False)
-        return rope._turn(tokens, keys, positions, inverse)
+        out = rope._turn(tokens, keys, positions, inverse)
+        if still is not None:
+            ctx.mark_non_differentiable(out[still])
+        return out
 
     @staticmethod
     def backward(ctx, g_tokens, g_keys=None):
         (positions,) = ctx.saved_tensors
-        return (None, None, None) + ctx.rope._turn_given(g_tokens, g_keys, positions, not ctx.inverse)
+        return (None, None, None) + ctx.rope._turn_given(g_tokens, g_keys, positions, not ctx.inverse) + (None,)
 
     @staticmethod
-    def jvp(ctx, _rope, _inverse, _positions, t_tokens, t_keys):
+    def jvp(ctx, _rope, _inverse, _positions, t_tokens, t_keys, _still=None):
         (positions,) = ctx.saved_tensors
         out = ctx.rope._turn_given(t_tokens, t_keys, positions, ctx.inverse)
         given = t_tokens if t_tokens is not None else t_keys
@@ -150,8 +153,8 @@ class RoPEAxes:
             positions = positions.to(tokens.device)
         if _has_tangent(positions):
             raise ValueError("RoPEAxes: no forward-mode derivative passes from the positions")
-        needs = (torch.is_grad_enabled() and (tokens.requires_grad or (keys is not None and keys.requires_grad))) or \
-            _has_tangent(tokens, keys)
+        tangent = _has_tangent(tokens, keys)
+        needs = tangent or (torch.is_grad_enabled() and (tokens.requires_grad or (keys is not None and keys.requires_grad)))
         if inplace:
             if needs:
                 raise ValueError("RoPEAxes: inplace rotation of a tensor that needs a gradient or has a forward-mode "
@@ -167,7 +170,10 @@ class RoPEAxes:
             self._run(tokens, keys, positions, False, tokens, keys)
             return tokens if keys is None else (tokens, keys)
         if needs:
-            out = _RoPEAxesTurn.apply(self, False, positions.detach(), tokens, keys)
+            still = None  # keys that need no gradient come back so beside tokens that do, and the other way round
+            if not tangent and keys is not None and tokens.requires_grad != keys.requires_grad:
+                still = 1 if tokens.requires_grad else 0
+            out = _RoPEAxesTurn.apply(self, False, positions.detach(), tokens, keys, still)
         else:
             out = self._turn(tokens, keys, positions, False)
         return out[0] if keys is None else out

@@ -105,3 +105,19 @@ def test_what_has_no_derivative_is_refused(turn, device):
         with pytest.raises(ValueError, match="positions"):
             turn(q, fwd.make_dual(where, torch.ones_like(where)))
     assert torch.equal(q, before)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_only_what_needs_a_gradient_gets_one(turn, device, which):
+    """Keys that need no gradient come back so beside tokens that do (a cache takes them), and the other way round."""
+    x = [_x(device, 3, 1), _x(device, 2, 2)]
+    pos, up = _pos(device), _x(device, 3 - which, 6)
+    x[which].requires_grad_()
+    out = turn(x[0], pos, x[1])
+    assert out[which].requires_grad and not out[1 - which].requires_grad
+    (g,) = torch.autograd.grad(out[which], x[which], up)
+    _check(g, up, pos, "gradient", inverse=True)
+    with fwd.dual_level():  # a tangent beside the gradient stays
+        x[1 - which] = fwd.make_dual(x[1 - which], torch.ones_like(x[1 - which]))
+        t = fwd.unpack_dual(turn(x[0], pos, x[1])[1 - which]).tangent
+        _check(t, torch.ones_like(t), pos, "tangent")
