@@ -12,6 +12,7 @@ import os
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libmapa.so")
 _lib = None
@@ -291,6 +292,13 @@ def on_device(device: torch.device):
     if device.index is None or device.index == torch.cuda.current_device():
         return _SAME_DEVICE
     return torch.cuda.device(device)
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether any of the tensors (or None) carries a forward-mode derivative."""
+    # outside a dual level none does: the level is looked at first (0.1 us; asking every tensor 0.3 each)
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                                  for t in tensors)
 
 
 def dt_code(dtype: torch.dtype) -> int:

@@ -140,6 +140,9 @@ class PagedKVCache:
         if t.requires_grad and torch.is_grad_enabled():
             raise nat.NativeError(f"PagedKVCache: {name} needs a gradient, and none passes through the cache "
                                   "(torch.no_grad() or detach())")
+        if nat.has_tangent(t):
+            raise nat.NativeError(f"PagedKVCache: {name} carries a forward-mode derivative, and none passes through the "
+                                  "cache")
 
     def _out(self, t: torch.Tensor, name: str, heads: int):
         self._rows(t, name, heads)
@@ -153,6 +156,9 @@ class PagedKVCache:
         if (self._k.requires_grad or self._v.requires_grad) and torch.is_grad_enabled():
             raise nat.NativeError("PagedKVCache: the pages need a gradient, and none passes through the cache "
                                   "(torch.no_grad() or detach())")
+        if nat.has_tangent(self._k, self._v):
+            raise nat.NativeError("PagedKVCache: the pages carry a forward-mode derivative, and none passes through the "
+                                  "cache")
 
     def write(self, k: torch.Tensor, v: torch.Tensor, batch: KVBatch):
         """The batch's new keys and values (rows, heads, 64), fp32, bf16 or fp16, into their pages.  Rows behind the

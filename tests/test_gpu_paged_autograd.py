@@ -2,6 +2,7 @@
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 from test_gpu_paged import E4M3, Scene, _ints, _randn, nat, no_fault  # noqa: F401  (fixtures)
 
@@ -48,3 +49,25 @@ def test_pages_that_need_a_gradient_are_refused(nat, which):
                 call()
             with torch.no_grad():
                 call()
+
+
+def test_forward_mode_derivatives_are_refused(nat):
+    from mapanything.kv_cache import PagedKVCache
+
+    s = Scene([(2, 40)], 2, 16, torch.bfloat16)
+    s.fill(1)
+    rows = _randn(2, 2, 64, seed=2, dtype=torch.bfloat16)
+    cu = _ints([0, 40])
+    bufs = [torch.zeros(40, 2, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    want = s.cache.attend(rows, s.batch)
+    with fwd.dual_level():
+        dual = fwd.make_dual(rows, torch.ones_like(rows))
+        wide = fwd.make_dual(bufs[1], torch.ones_like(bufs[1]))
+        held = PagedKVCache.wrap(fwd.make_dual(s.cache.k, torch.ones_like(s.cache.k)), s.cache.v)
+        for call in (lambda: s.cache.attend(dual, s.batch), lambda: s.cache.write(dual, rows, s.batch),
+                     lambda: s.cache.write(rows, dual, s.batch), lambda: s.cache.attend(rows, s.batch, out=dual),
+                     lambda: s.cache.read(s.batch, cu, 40, out=(bufs[0], wide)), lambda: held.attend(rows, s.batch),
+                     lambda: held.read(s.batch, cu, 40)):
+            with pytest.raises(nat.NativeError, match="forward-mode"):
+                call()
+        assert torch.equal(s.cache.attend(rows, s.batch), want)  # tensors without one, at the same level
