@@ -512,7 +512,8 @@ int mapa_rope_axes(const mapa_rope_axes_desc* d, mapa_stream_t stream);
  * mapa_kv_cache_write: new rows k, v (f32 / bf16 / f16; element strides of row and head, contiguous 64) into their
  *   pages.  A page that the call writes stands in the table once (two tokens of one place: either's row).
  * mapa_kv_cache_read: positions 0 .. cu_rows[b + 1] - cu_rows[b] - 1 of every sequence to the packed rows from
- *   cu_rows[b] on (k_out, v_out [rows][heads][64] with element strides, f32 / bf16 / f16); positions past kv_lens[b]
+ *   cu_rows[b] on (k_out, v_out [rows][heads][64] with element strides, f32 / bf16 / f16; they share nothing, one
+ *   pointer for both is refused); positions past kv_lens[b]
  *   read as zero, rows from cu_rows[seqs] on are left as they are. */
 typedef struct {
   int dtype;

@@ -365,6 +365,7 @@ extern "C" int mapa_kv_cache_read(const mapa_kv_cache* c, const mapa_kv_batch* b
                          "mapa_kv_cache_read"))
     return rc;
   MAPA_CHECK_ARG(cu_rows != nullptr, "mapa_kv_cache_read: null cu_rows");
+  MAPA_CHECK_ARG(k_out != v_out, "mapa_kv_cache_read: keys and values have one output");
   a.cu = cu_rows;
   a.rows = rows;
   a.tb = tokens_per_block(a.rows);

@@ -176,7 +176,8 @@ class PagedKVCache:
 
     def read(self, batch: KVBatch, cu_rows: torch.Tensor, rows: int, dtype: torch.dtype = torch.bfloat16, out=None):
         """(k, v), (rows, heads, 64) each: positions 0, 1, ... of sequence b in the rows cu_rows[b] .. cu_rows[b + 1] -
-        1, positions past kv_lens[b] as zeros; rows behind the last sequence stay as they are in `out`."""
+        1, positions past kv_lens[b] as zeros; rows behind the last sequence stay as they are in `out`, a (k, v) pair of
+        tensors that share nothing."""
         self._same(batch)
         _int32(cu_rows, "PagedKVCache: cu_rows", 1)
         if cu_rows.shape[0] != batch._cu_new.shape[0] or cu_rows.device != self._k.device:
