@@ -510,7 +510,8 @@ int mapa_rope_axes(const mapa_rope_axes_desc* d, mapa_stream_t stream);
  * tokens / cached tokens.  All three arrays are int32 device memory; what they hold is checked on the device
  * (MAPA_FAULT_KV_RANGE).
  * mapa_kv_cache_write: new rows k, v (f32 / bf16 / f16; element strides of row and head, contiguous 64) into their
- *   pages.  A page that the call writes stands in the table once (two tokens of one place: either's row).
+ *   pages.  A page that the call writes stands in the table once (two tokens of one place: either's row).  Pages that
+ *   keys and values share (k == v) can be read and attended over, a write refuses them.
  * mapa_kv_cache_read: positions 0 .. cu_rows[b + 1] - cu_rows[b] - 1 of every sequence to the packed rows from
  *   cu_rows[b] on (k_out, v_out [rows][heads][64] with element strides, f32 / bf16 / f16; they share nothing, one
  *   pointer for both is refused); positions past kv_lens[b]

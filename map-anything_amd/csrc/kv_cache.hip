@@ -338,6 +338,9 @@ extern "C" int mapa_kv_cache_write(const mapa_kv_cache* c, const mapa_kv_batch* 
   }
   if (int rc = fill_args(a, c, b, k, v, dtype, k_rstride, k_hstride, v_rstride, v_hstride, "mapa_kv_cache_write"))
     return rc;
+  const bool codes = c->dtype == MAPA_FP8 || c->dtype == MAPA_I8;
+  MAPA_CHECK_ARG(c->k != c->v && !(codes && c->k_exp == c->v_exp),
+                 "mapa_kv_cache_write: keys and values share their pages or exponents");
   a.cu = b->cu_new;
   a.rows = b->new_rows;
   a.tb = tokens_per_block(a.rows);
