@@ -65,6 +65,8 @@ class KVBatch:
             max_new = int((cu_new[1:] - cu_new[:-1]).max()) if seqs else 0
         if max_kv is None:
             max_kv = int(kv_lens.max()) if seqs else 0
+        if not (0 <= max_new < 1 << 31 and 0 <= max_kv <= 1 << 30):  # (a C int would take what is left of a larger one)
+            raise nat.NativeError(f"KVBatch: max_new {max_new} and max_kv {max_kv} must be 0 to 2^31 - 1 and 0 to 2^30")
         self._table, self._kv_lens, self._cu_new, self._max_new, self._max_kv = table, kv_lens, cu_new, max_new, max_kv
         # a one-row table's stride says nothing, its width does
         width = table.shape[1]
@@ -207,6 +209,10 @@ class PagedKVCache:
         return_lse: also (query heads, rows) fp32 log-sum-exp, as `_native.attn_merge` takes it."""
         self._rows(q, "q")
         self._same(batch)
+        if not 0 <= mask_block < 1 << 31:
+            raise nat.NativeError(f"PagedKVCache: mask_block {mask_block} must be 0 to 2^31 - 1")
+        if scale and not 2.0 ** -149 <= scale < 1e30:  # (less is fp32's zero, which means the default)
+            raise nat.NativeError(f"PagedKVCache: scale {scale} must be positive, 2^-149 to 1e30, or None")
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
         else:
