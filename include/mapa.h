@@ -53,7 +53,7 @@ int mapa_device_check(int device);
  * HIP_LAUNCH_BLOCKING is set) — SURVEY.md §5's race-detection / serialize row; no reference counterpart. */
 int mapa_stream_check(mapa_stream_t stream, const char* what);
 
-/* Device-side fault channel (round 5).  Kernels that can detect a failed assumption at run time set a bit of the
+/* Device-side fault channel.  Kernels that can detect a failed assumption at run time set a bit of the
  * library's sticky fault word (below) instead of hanging or failing silently; today one: MAPA_FAULT_LN_BARRIER, a
  * LayerNorm-fused GEMM band barrier (mapa_gemm_desc.ln_out) that did not complete within its bounded wait — that
  * launch's LayerNorm rows are invalid.
@@ -63,12 +63,13 @@ int mapa_stream_check(mapa_stream_t stream, const char* what);
  *     every earlier launch on the stream has completed (graph-capturable).  The host zeroes slot[0], enqueues the
  *     work and the publish, and polls slot[0] != 0 — no stream synchronisation, so the GPU keeps running the work
  *     queued after the publish (MapAnything.infer publishes after the transformer and checks before returning).
- *   mapa_fault_reset: enqueue on `stream` a kernel that clears the fault word once every earlier launch on the
- *     stream has completed (graph-capturable); MapAnything.infer / forward start every call with it, so a publish
- *     reports only faults of its own call.
+ *   mapa_fault_reset: enqueue on `stream` a kernel that clears the forward's bits (MAPA_FAULT_LN_BARRIER and
+ *     MAPA_FAULT_F16_RANGE) once every earlier launch on the stream has completed (graph-capturable);
+ *     MapAnything.infer / forward start every call with it, so a publish reports of them only its own call's.
+ *     MAPA_FAULT_KV_RANGE stays until mapa_fault_status resets it; the forward does not go by it.
  *   mapa_fault_status: synchronous read of the fault word (and reset to 0 when `reset`); -1 on a HIP error.
  *   mapa_stream_check also reports and clears it.
- * The word is per device and per calling host thread (round 6: a thread's word is fixed at its first library call;
+ * The word is per device and per calling host thread (a thread's word is fixed at its first library call;
  * 64 words, threads beyond share round robin): every launch, reset, publish and status call of a thread uses its own
  * word, so concurrent callers on different streams of one process (one thread each) neither see nor clear each
  * other's faults.  A captured graph keeps the word of the thread that captured it.  The library's cached device

@@ -145,8 +145,10 @@ bool launch_gemm_big_ln(const GemmArgs& a, int variant, void* ws, int64_t ws_byt
 }
 
 // The calling thread's fault word: stream-ordered reset and publish into a host-visible slot, synchronous read / reset.
+// A forward starts with the reset, which leaves what a paged K/V cache call reported before it (MAPA_FAULT_KV_RANGE).
+constexpr unsigned FORWARD_FAULTS = MAPA_FAULT_LN_BARRIER | MAPA_FAULT_F16_RANGE;
 __global__ void fault_reset_kernel(unsigned* word) {
-  if (threadIdx.x == 0) __hip_atomic_store(word, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (threadIdx.x == 0) __hip_atomic_fetch_and(word, ~FORWARD_FAULTS, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 __global__ void fault_publish_kernel(const unsigned* word, unsigned* slot) {

@@ -43,6 +43,7 @@ EXPORTED = (
 FAULT_LN_BARRIER = 1  # include/mapa.h MAPA_FAULT_LN_BARRIER
 FAULT_F16_RANGE = 2  # include/mapa.h MAPA_FAULT_F16_RANGE
 FAULT_KV_RANGE = 4  # include/mapa.h MAPA_FAULT_KV_RANGE
+ENGINE_FAULTS = FAULT_LN_BARRIER | FAULT_F16_RANGE  # a forward's own: what mapa_fault_reset clears
 ROPE_AXIAL, ROPE_HALF, ROPE_INTERLEAVED = 0, 1, 2  # include/mapa.h MAPA_ROPE_*
 POS_I64, POS_F32 = 0, 1  # include/mapa.h MAPA_POS_*
 ROPE_MAX_AXES, ROPE_MAX_PAIRS = 4, 128
@@ -334,10 +335,13 @@ def fault_status(reset: bool = True) -> int:
     return v
 
 
-def check_faults():
-    """Raise NativeError if a kernel set the device fault word since the last check (synchronises the device)."""
-    v = fault_status(reset=True)
+def check_faults(bits: Optional[int] = None):
+    """Raise NativeError if a kernel launched by this thread set the device fault word since the last check
+    (synchronises the device).  bits: ENGINE_FAULTS for a forward's alone, which leaves a paged cache's to be told."""
+    v = fault_status(reset=bits is None) & (-1 if bits is None else bits)
     if v:
+        if bits is not None:
+            FaultSlot.reset()
         raise DeviceFault(v)
 
 
@@ -346,7 +350,8 @@ class FaultTimeout(NativeError):
 
 
 class FaultSlot:
-    """A host-visible slot the device writes its fault word into, stream-ordered (mapa_fault_publish): the host
+    """A host-visible slot the device writes its fault word into, stream-ordered (mapa_fault_publish), for a forward's
+    own faults (ENGINE_FAULTS; a paged cache's stay in the word for check_faults): the host
     arms it (slot = 0), enqueues work + publish(), and wait() polls the slot — without synchronising the stream, so
     the kernels queued after the publish keep the GPU busy while the host checks.  One slot per captured graph (its
     publish node is baked into the graph with this slot's address) and one per eager caller."""
@@ -373,11 +378,12 @@ class FaultSlot:
 
     @staticmethod
     def reset():
-        """Enqueue the fault word's reset on the current stream (the start of a call; also inside a capture)."""
+        """Enqueue the reset of the fault word's ENGINE_FAULTS on the current stream (the start of a call; also inside a
+        capture)."""
         check(lib().mapa_fault_reset(stream()), "mapa_fault_reset")
 
     def wait(self, timeout_s: float = 600.0, poll=None):
-        """Poll until the armed publish has run; raise NativeError if it carried a fault (the device word is reset).
+        """Poll until the armed publish has run; raise NativeError if it carried a fault (the reset is enqueued).
         The poll sleeps ~50 us between reads, calls `poll()` (e.g. a communicator's asynchronous-error check) every
         ~10 ms, and raises FaultTimeout past timeout_s, or NativeError if the stream drains without the publish."""
         import time
@@ -403,9 +409,9 @@ class FaultSlot:
                 poll()
                 t_poll = now
             time.sleep(5e-5)
-        bits = v >> 1
+        bits = (v >> 1) & ENGINE_FAULTS
         if bits:
-            fault_status(reset=True)
+            self.reset()
             raise DeviceFault(bits)
 
     def __del__(self):

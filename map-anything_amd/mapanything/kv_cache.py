@@ -11,7 +11,8 @@ sequence), 16-bit or quantised as they are written.  Head width is 64, as in eve
     out = cache.attend(q, batch, mask_block=1370)            # every view sees itself and the earlier ones
 
 No CPU path: a missing library or device raises.  Page numbers, lengths and offsets live in device memory and are
-checked there: `_native.check_faults()` raises if a call met one outside the cache."""
+checked there: `_native.check_faults()` raises if a call of its thread (or a graph that the thread captured) met one
+outside the cache since the last check, whatever ran in between."""
 
 from __future__ import annotations
 
