@@ -215,19 +215,6 @@ __device__ __forceinline__ RowTile find_tile(const PagedArgs& p, int tile, int l
   }
   return RowTile{-1, 0, 0, 0, 0};
 }
-// place j of n things taken in `classes` passes over every classes-th one (the first n % classes passes have one more)
-__device__ __forceinline__ int pass_order(int j, int n, int classes) {
-  if (classes == 1) return j;
-  const int least = n / classes, more = n - least * classes, cut = more * (least + 1);
-  const int len = j < cut ? least + 1 : least, in = j < cut ? j : j - cut, pass = in / len;
-  return pass + (j < cut ? 0 : more) + classes * (in - pass * len);
-}
-// task of the chunk kernel -> (K/V head, row tile): row tiles inside heads (they share K/V), the last ones (the longest
-// key ranges under a causal mask) first, in passes
-__device__ __forceinline__ void task_coords(const PagedArgs& p, int task, int& hk, int& tile) {
-  hk = task / p.tiles;
-  tile = p.tiles - 1 - pass_order(task - hk * p.tiles, p.tiles, p.tile_passes);
-}
 
 // ------------------------------------------------------------------------------------------------ chunk
 // CK: 0 = 16-bit pages of the query's type, 1 = e4m3, 2 = int8.  NW: waves of a workgroup, 32 rows each (the plan's rule
@@ -241,25 +228,9 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_paged_chunk(PagedArgs p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hl = lane >> 5, l32 = lane & 31;
 
-  // whole tasks first, each XCD a contiguous run of them; then the split ones, where workgroups that share a K/V range
-  // run together on one XCD: (head, range, row tile) if all tasks are split — ranges outermost would give one XCD the
-  // last ranges, which only the longest sequence has (ragged causal int8 chunks: 201 us so, 142 us head by head) — and
-  // (range, task) for the rest of one sequence's tasks
-  int task, split = 0, slot = -1;
-  if ((int)blockIdx.x < p.whole) {
-    task = mapa_idx::xcd_remap(blockIdx.x, p.whole);
-  } else {
-    const int rest = p.tiles * p.kv_heads - p.whole;
-    const int v = mapa_idx::xcd_remap(blockIdx.x - p.whole, rest * p.splits);
-    const int per = p.whole ? rest : p.tiles;
-    const int group = v / (per * p.splits), in = v - group * per * p.splits;
-    const int nth = in / per, j = group * per + in - nth * per;
-    split = pass_order(nth, p.splits, p.range_passes);
-    task = p.whole + j;
-    slot = j * p.splits + split;
-  }
-  int hk, tile;
-  task_coords(p, task, hk, tile);
+  int task, split, slot, hk, tile;
+  mapa_idx::paged_chunk_work(blockIdx.x, p.whole, p.tiles, p.kv_heads, p.splits, p.range_passes, task, split, slot);
+  mapa_idx::paged_task(task, p.tiles, p.tile_passes, hk, tile);
   const RowTile rt0 = find_tile(p, tile, lane);
   const int b = rt0.seq, nq = rt0.nq, c0 = rt0.c0, len = rt0.len;
   tile = rt0.tile;
@@ -720,8 +691,8 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, l16 = lane & 15;
 
-  // (sequence, key range, K/V head): the heads of a range innermost, so that one table row serves neighbours
-  const int hk = blockIdx.x % p.kv_heads, bs = blockIdx.x / p.kv_heads, split = bs % p.splits, b = bs / p.splits;
+  int b, split, hk;
+  mapa_idx::paged_step_work(blockIdx.x, p.kv_heads, p.splits, b, split, hk);
   // The page window and, for one sequence alone, the first tiles are fetched before its length is known (the range's
   // place is not a matter of it; what lies past the sequence is hidden later): one trip to memory less in a chain of
   // four.  Of several sequences most ranges may be past the end, and other workgroups cover the wait.  Pages are held
@@ -1016,7 +987,7 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
           uint2{pack16<F16>(v[0], v[1]), pack16<F16>(v[2], v[3])};
       if (p.lse && d == 0) p.lse[(int64_t)h * p.new_rows + t] = lse2 * LN2;
     } else {
-      const int64_t pr = (((int64_t)b * p.kv_heads + hk) * p.splits + split) * RS + row;
+      const int64_t pr = mapa_idx::paged_step_slot(b, hk, split, p.kv_heads, p.splits) * RS + row;
       *reinterpret_cast<f32x4*>(p.part_o + pr * HD + d) = v;
       if (d == 0) p.part_lse[pr] = lse2;
     }
@@ -1109,7 +1080,7 @@ __global__ void __launch_bounds__(NT) attn_paged_merge_chunk(PagedArgs p) {
   const int lane = threadIdx.x & 63, d = (threadIdx.x & 15) * 4;
   const int j = blockIdx.x;
   int hk, tile;
-  task_coords(p, p.whole + j, hk, tile);
+  mapa_idx::paged_task(p.whole + j, p.tiles, p.tile_passes, hk, tile);
   const RowTile rt = find_tile(p, tile, lane);
   if (rt.seq < 0) return;
   const int len = rt.len;
@@ -1151,7 +1122,7 @@ __global__ void __launch_bounds__(NT) attn_paged_merge_step(PagedArgs p) {
   constexpr int RS = RB * 16;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = blockIdx.x / p.kv_heads, hk = blockIdx.x - b * p.kv_heads, r = blockIdx.y * 4 + wave;
-  const int64_t first = (int64_t)blockIdx.x * p.splits * RS + r;
+  const int64_t first = mapa_idx::paged_step_slot(b, hk, 0, p.kv_heads, p.splits) * RS + r;
   Ranges part;
   load_ranges<RS>(p, first, 0, lane, part);
   const int c0 = p.cu[b];

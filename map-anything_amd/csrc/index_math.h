@@ -180,6 +180,55 @@ MAPA_HD void attn_block_work(int bid, int n_dp, int chunks, int nkt, int& task, 
   }
 }
 
+// ---- paged attention (attention_paged.hip)
+// Place j of n things taken in `classes` passes over every classes-th one (the first n % classes passes have one more).
+MAPA_HD int pass_order(int j, int n, int classes) {
+  if (classes == 1) return j;
+  const int least = n / classes, more = n - least * classes, cut = more * (least + 1);
+  const int len = j < cut ? least + 1 : least, in = j < cut ? j : j - cut, pass = in / len;
+  return pass + (j < cut ? 0 : more) + classes * (in - pass * len);
+}
+// Task of the chunk kernel -> (K/V head, row tile): row tiles inside heads (they share K/V), the last ones (the longest
+// key ranges under a causal mask) first, in passes.
+MAPA_HD void paged_task(int task, int tiles, int tile_passes, int& hk, int& tile) {
+  hk = task / tiles;
+  tile = tiles - 1 - pass_order(task - hk * tiles, tiles, tile_passes);
+}
+// Work of the chunk kernel's block bid: the tasks below `whole` walk all their keys (slot -1), the others' keys are cut
+// into `splits` ranges with a slot of partials each, task whole + j's from slot j * splits on.  Whole tasks first, each
+// XCD a contiguous run of them; then the split ones, where workgroups that share a K/V range run together on one XCD:
+// (head, range, row tile) if all tasks are split — ranges outermost would give one XCD the last ranges, which only the
+// longest sequence has (ragged causal int8 chunks: 201 us so, 142 us head by head) — and (range, task) for the rest of
+// one sequence's tasks.
+MAPA_HD void paged_chunk_work(int bid, int whole, int tiles, int heads, int splits, int range_passes, int& task,
+                              int& split, int& slot) {
+  if (bid < whole) {
+    task = xcd_remap(bid, whole);
+    split = 0;
+    slot = -1;
+    return;
+  }
+  const int rest = tiles * heads - whole;
+  const int v = xcd_remap(bid - whole, rest * splits);
+  const int per = whole ? rest : tiles;
+  const int group = v / (per * splits), in = v - group * per * splits;
+  const int nth = in / per, j = group * per + in - nth * per;
+  split = pass_order(nth, splits, range_passes);
+  task = whole + j;
+  slot = j * splits + split;
+}
+// Block of the step kernel -> (sequence, key range, K/V head): the heads of a range innermost, so that one table row
+// serves neighbours; its slot of partials.
+MAPA_HD void paged_step_work(int bid, int heads, int splits, int& seq, int& split, int& hk) {
+  const int bs = bid / heads;
+  hk = bid - bs * heads;
+  seq = bs / splits;
+  split = bs - seq * splits;
+}
+MAPA_HD int64_t paged_step_slot(int seq, int hk, int split, int heads, int splits) {
+  return ((int64_t)seq * heads + hk) * splits + split;
+}
+
 // ---- halo conv (conv_halo.hip): block id -> (image, block row, block col, column tile)
 MAPA_HD void halo_block(int bid, int imgs, int nby, int nbx, int ntn, int& img, int& by, int& bx, int& tn) {
   int t = xcd_remap(bid, imgs * nby * nbx * ntn);

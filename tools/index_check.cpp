@@ -10,6 +10,9 @@
 //     exactly sk_contributors' range, slab slots stay inside the g slab pairs of the workspace, the grid fits g;
 //   * attention: every task's K/V tile range [0, nkt) is covered exactly once by its chunks, chunks are non-empty,
 //     partial slots stay inside the workspace's `slots` rows;
+//   * paged attention: passes are permutations; every (task, key range) of the chunk kernel and every (sequence, head,
+//     key range) of the step kernel is taken by exactly one block, slots of partials are each written once, inside
+//     the workspace, where the merge looks for them;
 //   * the halo-conv block decode visits every (image, block row, block col, column tile) once;
 //   * the conv K-column decode is a bijection onto (tap, channel) for every K order;
 //   * the clamped grid-stride step never passes `total`, even one grid short of 2^31.
@@ -129,6 +132,50 @@ static void check_attention(int ntask, int nkt, int slots) {
     next_k[task] = k1;
   }
   for (int t = 0; t < ntask; ++t) REQUIRE(next_k[t] == nkt, "task %d covered to %d of %d", t, next_k[t], nkt);
+}
+
+// A plan of attention_paged.hip: `whole` of tiles * heads tasks walk all keys, the others `splits` ranges each
+static void check_paged_chunk(int tiles, int heads, int whole, int splits, int tile_passes, int range_passes) {
+  const int tasks = tiles * heads;
+  std::vector<char> seen(tasks, 0);
+  for (int t = 0; t < tasks; ++t) {
+    int hk, tile;
+    paged_task(t, tiles, tile_passes, hk, tile);
+    REQUIRE(hk >= 0 && hk < heads && tile >= 0 && tile < tiles, "task %d -> (%d, %d)", t, hk, tile);
+    REQUIRE(!seen[hk * tiles + tile], "task %d: (%d, %d) again", t, hk, tile);
+    seen[hk * tiles + tile] = 1;
+  }
+  const int slots = splits > 1 ? (tasks - whole) * splits : 0, grid = whole + (tasks - whole) * splits;
+  std::vector<char> taken((size_t)tasks * splits, 0), written(slots, 0);
+  for (int b = 0; b < grid; ++b) {
+    int task, split, slot;
+    paged_chunk_work(b, whole, tiles, heads, splits, range_passes, task, split, slot);
+    REQUIRE(task >= 0 && task < tasks && split >= 0 && split < splits, "block %d -> task %d range %d", b, task, split);
+    REQUIRE((slot < 0) == (task < whole), "block %d: task %d of %d whole, slot %d", b, task, whole, slot);
+    char& t = taken[(size_t)task * splits + split];
+    REQUIRE(!t, "task %d range %d again", task, split);
+    t = 1;
+    if (slot >= 0) {
+      REQUIRE(slot == (task - whole) * splits + split, "slot %d of task %d range %d", slot, task, split);
+      REQUIRE(slot < slots && !written[slot], "slot %d of %d", slot, slots);
+      written[slot] = 1;
+    }
+  }
+  for (int t = 0; t < tasks; ++t)
+    for (int s = 0; s < (t < whole ? 1 : splits); ++s) REQUIRE(taken[(size_t)t * splits + s], "task %d range %d left out", t, s);
+}
+
+static void check_paged_step(int seqs, int heads, int splits) {
+  std::vector<char> written((size_t)seqs * heads * splits, 0);
+  for (int b = 0; b < seqs * heads * splits; ++b) {
+    int seq, split, hk;
+    paged_step_work(b, heads, splits, seq, split, hk);
+    REQUIRE(seq >= 0 && seq < seqs && split >= 0 && split < splits && hk >= 0 && hk < heads, "block %d", b);
+    const int64_t slot = paged_step_slot(seq, hk, split, heads, splits);
+    REQUIRE(slot == paged_step_slot(seq, hk, 0, heads, splits) + split, "slot %ld", (long)slot);
+    REQUIRE(slot >= 0 && slot < (int64_t)written.size() && !written[slot], "slot %ld", (long)slot);
+    written[slot] = 1;
+  }
 }
 
 static void check_halo(int imgs, int nby, int nbx, int ntn) {
@@ -256,6 +303,24 @@ int main() {
   for (int sl : slots)
     for (const A& a : att) check_attention(((a.seq_q + 127) / 128) * a.heads * a.batch, (a.seq_kv + 63) / 64, sl);
   for (int i = 0; i < 3000; ++i) check_attention(1 + rng() % 6000, 1 + rng() % 50000, 1 + rng() % 1200);
+
+  // paged attention: one view and eight over 12, 16, 48 heads on 512 or 256 slots (mixed, all whole, all split), random
+  for (int tiles : {1, 6, 11, 43, 86, 90})
+    for (int heads : {1, 4, 12, 16, 48})
+      for (int resident : {512, 256})
+        for (int splits : {2, 3, 58, 64})
+          for (int passes : {1, 2, 4, 8}) {
+            const int tasks = tiles * heads, whole = tasks / resident * resident;
+            const int tp = imin(passes, tiles), rp = imin(passes, splits);
+            check_paged_chunk(tiles, heads, whole, whole == tasks ? 1 : splits, tp, imin(rp, whole == tasks ? 1 : splits));
+            check_paged_chunk(tiles, heads, tasks, 1, tp, 1);
+            check_paged_chunk(tiles, heads, 0, splits, 1, rp);
+          }
+  for (int i = 0; i < 2000; ++i) {
+    const int tiles = 1 + rng() % 60, heads = 1 + rng() % 24, splits = 2 + rng() % 20;
+    check_paged_chunk(tiles, heads, rng() % (tiles * heads), splits, 1 + rng() % imin(8, tiles), 1 + rng() % imin(8, splits));
+    check_paged_step(1 + rng() % 40, 1 + rng() % 24, 1 + rng() % 20);
+  }
 
   // halo conv blocks: 16x16 (or 8x16) pixel blocks of the 518 / 296 / 148 maps, 128 / 256-wide column tiles
   const int maps[] = {518, 296, 148, 74, 37};
