@@ -1180,15 +1180,18 @@ int ragged_splits(int64_t tasks, int tiles, int slots, double fixed, int most) {
   return std::max(1, std::min({most, tiles, (int)(n + 0.5)}));
 }
 
-// Waves of a chunk workgroup (32 rows each).  Eight share a tile's decoding where two workgroups of four do it twice: an
-// 8-view chunk over int8 pages takes 729 us with eight and 785 with four (e4m3 691 and 706), a 1370-token view over 100
-// views 717 and 767 (680 and 693) though a twelfth of its eight-wave rows is empty.  16-bit pages have nothing to decode
-// (642 and 633 us, 656 and 659), and ragged batches want the finer pieces (ragged causal int8 chunks 133 and 122 us).
+// Waves of a chunk workgroup (32 rows each).  Eight share a tile's decoding where two workgroups of four do it twice, and
+// leave more rows of the last tile empty.  One sequence over 12 heads and 55 thousand keys, eight against four waves, by
+// the ratio of their padded rows: int8 pages 0.83 to 0.91 of the time at 1 to 1.11 (1370 rows 308 and 340 us), 0.96 at
+// 1.14, 0.99 at 1.2, 1.10 at 1.33; e4m3, cheaper to decode, 0.89 to 0.97 at 1 to 1.11 (291 and 304 us), 1.03 at 1.14, 1.15
+// at 1.33; over 6 thousand keys eight are no slower anywhere.  16-bit pages have nothing to decode (an 8-view chunk 642
+// and 633 us), and ragged batches want the finer pieces (ragged causal int8 chunks 133 and 122 us).
 int chunk_waves(const mapa_attn_paged_desc& d) {
-  const bool codes = d.cache.dtype == MAPA_FP8 || d.cache.dtype == MAPA_I8;
   const int64_t rows = (int64_t)d.batch.max_new * (d.heads / d.cache.heads);
   const int64_t four = (rows + 127) / 128 * 128, eight = (rows + 255) / 256 * 256;
-  return codes && d.batch.seqs == 1 && eight * 10 <= four * 11 ? 8 : 4;
+  if (d.batch.seqs != 1) return 4;
+  if (d.cache.dtype == MAPA_I8) return eight * 5 <= four * 6 ? 8 : 4;
+  return d.cache.dtype == MAPA_FP8 && eight * 8 <= four * 9 ? 8 : 4;
 }
 
 // Passes over a head's row tiles or key ranges: as many as cut it where the 8 XCDs' equal runs of the work end, so that an

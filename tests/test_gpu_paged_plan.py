@@ -1,5 +1,5 @@
-"""Attention over a paged cache under the plan that walks most tasks whole and cuts the rest of one sequence's tasks into
-key ranges."""
+"""Attention over a paged cache under its plans: most tasks whole and the rest of one sequence's cut into key ranges; four
+or eight waves a workgroup."""
 
 import ctypes
 
@@ -30,5 +30,18 @@ def test_whole_and_split_tasks_of_one_sequence(nat, kind, pages, waves, block, n
     assert tasks > resident and slots == int(slots) and slots >= 2 * rest and slots % rest == 0 and slots < 2 * tasks
     got, lse = s.cache.attend(q, s.batch, mask_block=block, return_lse=True)
     want, wlse, tol, ltol = s.expect(q, block)
+    ref.within(got, want, tol, "out")
+    ref.within(lse, wlse, ltol, "lse")
+
+
+@pytest.mark.parametrize("kind,pages", [(torch.bfloat16, E4M3), (torch.float16, torch.int8)], ids=str)
+@pytest.mark.parametrize("new", [100, 130, 300, 500, 600, 860, 1100])
+def test_either_number_of_waves(nat, kind, pages, new):
+    """Rows that pad to as many, a few or many more in workgroups of 256 than of 128, on both sides of the rule."""
+    s = Scene([(new, 2500)], 2, 64, pages)
+    s.fill(3, kind)
+    q = _randn(new, 2, 64, seed=5, dtype=kind)
+    got, lse = s.cache.attend(q, s.batch, mask_block=1, return_lse=True)
+    want, wlse, tol, ltol = s.expect(q, 1)
     ref.within(got, want, tol, "out")
     ref.within(lse, wlse, ltol, "lse")
