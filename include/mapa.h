@@ -272,7 +272,8 @@ int64_t mapa_attention_workspace_bytes(const mapa_attn_desc* d);
 /* Merge two attention partials of the same queries over disjoint key sets using their LSEs (the sharded global
  * layer overlaps its K/V all-gather with the local-key partial): o = (e^{lse_a} o_a + e^{lse_b} o_b) /
  * (e^{lse_a} + e^{lse_b}).  o_* [rows][heads*64] (row stride ld, bf16 or f32 per dtype; o_out may alias o_a),
- * lse_* [heads][rows] natural-log f32 as mapa_attention writes them (batch 1); lse_out optional. */
+ * lse_* [heads][rows] natural-log f32 as mapa_attention writes them (batch 1); lse_out optional.  Two lse of -inf (a row
+ * that sees nothing in either part) give zeros and -inf. */
 int mapa_attn_merge(const void* o_a, const float* lse_a, const void* o_b, const float* lse_b, void* o_out,
                     float* lse_out, int dtype, int rows, int heads, int64_t ld, mapa_stream_t stream);
 

@@ -619,9 +619,9 @@ __global__ void attn_merge_kernel(const T* __restrict__ oa, const float* __restr
     const int h = (int)(rh % heads);
     const int r = (int)(rh / heads);
     const float a = la[(int64_t)h * rows + r], b = lb[(int64_t)h * rows + r];
-    const float m = fmaxf(a, b);
-    const float wa = __expf(a - m), wb = __expf(b - m);
-    const float inv = 1.f / (wa + wb);
+    const float most = fmaxf(a, b), m = most == -INFINITY ? 0.f : most;  // -inf: neither part sees a key
+    const float wa = __expf(a - m), wb = __expf(b - m), sum = wa + wb;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const int64_t o = (int64_t)r * ld + h * 64 + d4;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -637,7 +637,7 @@ __global__ void attn_merge_kernel(const T* __restrict__ oa, const float* __restr
       if constexpr (sizeof(T) == 2) out[o + j] = f32_to_lp(F16, v);
       else out[o + j] = v;
     }
-    if (lse_out && d4 == 0) lse_out[(int64_t)h * rows + r] = m + __logf(wa + wb);
+    if (lse_out && d4 == 0) lse_out[(int64_t)h * rows + r] = m + __logf(sum);
   }
 }
 

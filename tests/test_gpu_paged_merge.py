@@ -38,3 +38,21 @@ def test_two_parts_join(nat, kind, pages, new, old, later):
     half = ref.half_step(kind)
     tol = w * ta + (1 - w) * tb + (a - b).abs() * w * (1 - w) * err + (a.abs() + b.abs()) * 2.0 ** -20
     ref.within(out, want, tol + half * (want.abs() + tol), "joined")
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+def test_parts_that_see_nothing(nat, kind):
+    """A row that sees nothing in one part is the other part's; in both, zeros and -inf, as attend gives them."""
+    rows, H = 6, 4
+    o = [_randn(rows, H, 64, seed=i, dtype=kind) for i in range(2)]
+    l = [_randn(H, rows, seed=7 + i) for i in range(2)]
+    for i, hidden in enumerate(((0, 1), (1, 2))):  # row 0: hidden in the first part, 1 in both, 2 in the second
+        for r in hidden:
+            o[i][r] = 0
+            l[i][:, r] = -float("inf")
+    out, lse = torch.empty_like(o[0]), torch.empty_like(l[0])
+    nat.attn_merge(o[0], l[0], o[1], l[1], out, rows, H, H * 64, lse_out=lse)
+    assert torch.equal(out[0], o[1][0]) and torch.equal(out[2], o[0][2]) and not out[1].any()
+    assert torch.equal(lse[:, 0], l[1][:, 0]) and torch.equal(lse[:, 2], l[0][:, 2])
+    assert (lse[:, 1] == -float("inf")).all()
+    assert torch.isfinite(out.float()).all()
