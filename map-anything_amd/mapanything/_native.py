@@ -960,11 +960,17 @@ def rope_axes(d: RopeAxesDesc):
     _toc(tok, "rope_axes")
 
 
+def _row_strides(t):
+    """Strides of the rows and heads of a (rows, heads, 64) tensor; of a single one torch's is arbitrary: none."""
+    (rows, heads, _), (rs, hs, _) = t.shape, t.stride()
+    return rs if rows > 1 else 0, hs if heads > 1 else 0
+
+
 def kv_cache_write(cache: KVCacheDesc, batch: KVBatchDesc, k, v):
     """New rows k, v (rows, heads, 64) into the pages of a paged K/V cache (mapanything.kv_cache.PagedKVCache)."""
     tok = _tic()
     check(lib().mapa_kv_cache_write(ctypes.byref(cache), ctypes.byref(batch), k.data_ptr(), v.data_ptr(),
-                                    dt_code(k.dtype), k.stride(0), k.stride(1), v.stride(0), v.stride(1), raw_stream()),
+                                    dt_code(k.dtype), *_row_strides(k), *_row_strides(v), raw_stream()),
           "mapa_kv_cache_write")
     _toc(tok, "kv_cache_write")
 
@@ -973,8 +979,8 @@ def kv_cache_read(cache: KVCacheDesc, batch: KVBatchDesc, cu_rows, rows: int, k,
     """Cached rows back into k, v (rows, heads, 64) (mapanything.kv_cache.PagedKVCache)."""
     tok = _tic()
     check(lib().mapa_kv_cache_read(ctypes.byref(cache), ctypes.byref(batch), cu_rows.data_ptr(), rows, k.data_ptr(),
-                                   v.data_ptr(), dt_code(k.dtype), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                                   raw_stream()), "mapa_kv_cache_read")
+                                   v.data_ptr(), dt_code(k.dtype), *_row_strides(k), *_row_strides(v), raw_stream()),
+          "mapa_kv_cache_read")
     _toc(tok, "kv_cache_read")
 
 
@@ -982,8 +988,9 @@ def attention_paged(cache: KVCacheDesc, batch: KVBatchDesc, q, o, *, lse=None, s
     """Attention of the batch's new tokens q (rows, heads, 64) over their sequences' pages.  The partials' workspace is
     a tensor of this call alone: the allocator orders its reuse on the current stream, and inside a graph capture it
     belongs to that graph's pool, so two graphs never share one."""
+    (qr, qh), (orr, oh) = _row_strides(q), _row_strides(o)
     d = AttnPagedDesc(cache=cache, batch=batch, dtype=dt_code(q.dtype), heads=q.shape[1], q=q.data_ptr(), o=o.data_ptr(),
-                      q_rstride=q.stride(0), q_hstride=q.stride(1), o_rstride=o.stride(0), o_hstride=o.stride(1),
+                      q_rstride=qr, q_hstride=qh, o_rstride=orr, o_hstride=oh,
                       lse=None if lse is None else lse.data_ptr(), scale=0.0 if scale is None else scale,
                       mask_block=mask_block)
     L = lib()

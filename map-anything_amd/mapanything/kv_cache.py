@@ -28,7 +28,7 @@ _PAGE_CODES = {torch.bfloat16: nat.BF16, torch.float16: nat.F16, torch.float8_e4
 
 
 def _int32(t: torch.Tensor, name: str, ndim: int) -> torch.Tensor:
-    if t.dtype != torch.int32 or t.ndim != ndim or not t.is_cuda or (t.numel() and t.stride(-1) != 1):
+    if t.dtype != torch.int32 or t.ndim != ndim or not t.is_cuda or not t.is_contiguous():
         raise nat.NativeError(f"{name}: a contiguous int32 GPU tensor with {ndim} dimension(s) is needed, got "
                               f"{t.dtype} {tuple(t.shape)} on {t.device}")
     return t
@@ -69,12 +69,8 @@ class KVBatch:
         if not (0 <= max_new < 1 << 31 and 0 <= max_kv <= 1 << 30):  # (a C int would take what is left of a larger one)
             raise nat.NativeError(f"KVBatch: max_new {max_new} and max_kv {max_kv} must be 0 to 2^31 - 1 and 0 to 2^30")
         self._table, self._kv_lens, self._cu_new, self._max_new, self._max_kv = table, kv_lens, cu_new, max_new, max_kv
-        # a one-row table's stride says nothing, its width does
-        width = table.shape[1]
-        if seqs > 1 and table.stride(0) != width:
-            raise nat.NativeError("KVBatch: table must be contiguous")
-        self.desc = nat.KVBatchDesc(seqs, width, table.data_ptr(), kv_lens.data_ptr(), cu_new.data_ptr(), 0, max_new,
-                                    max_kv)
+        self.desc = nat.KVBatchDesc(seqs, table.shape[1], table.data_ptr(), kv_lens.data_ptr(), cu_new.data_ptr(), 0,
+                                    max_new, max_kv)
 
     def _rows(self, rows: int) -> nat.KVBatchDesc:
         d = nat.KVBatchDesc.from_buffer_copy(self.desc)
