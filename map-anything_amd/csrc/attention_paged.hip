@@ -164,10 +164,10 @@ __device__ __forceinline__ bf16x8 part_of(bf16x8 v) {
   }
   return __builtin_bit_cast(bf16x8, uint4{w[0], w[1], w[2], w[3]});
 }
-// element j of 8 operand words, the others zero
-__device__ __forceinline__ bf16x8 only(bf16x8 v, int j) {
+// element j of 8 operand words if `on`, the others zero
+__device__ __forceinline__ bf16x8 only(bf16x8 v, int j, bool on) {
   const uint4 u = __builtin_bit_cast(uint4, v);
-  const uint32_t m = (j & 1) ? 0xffff0000u : 0xffffu;
+  const uint32_t m = !on ? 0u : (j & 1) ? 0xffff0000u : 0xffffu;
   const int w = j >> 1;
   const uint4 r = {w == 0 ? u.x & m : 0u, w == 1 ? u.y & m : 0u, w == 2 ? u.z & m : 0u, w == 3 ? u.w & m : 0u};
   return __builtin_bit_cast(bf16x8, r);
@@ -470,9 +470,10 @@ __global__ void __launch_bounds__(NW * 64, 2) attn_paged_chunk(PagedArgs p) {
         for (int fj = 0; fj < 64; ++fj) {
           const int f = fj >> 4, j = fj & 7, h2 = (fj >> 3) & 1;
           const int key = kt * KT + 16 * f + (j & 3) + 8 * (j >> 2) + 4 * h2;
-          const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
           const bf16x8 pr = f == 0 ? p0 : f == 1 ? p1 : f == 2 ? p2 : p3;
-          const bf16x8 pk = hl == h2 ? only(pr, j) : z, vk = hl == h2 ? only(part_of<F16, true>(v_frag(Vs, dt, f)), j) : z;
+          // (the transposed read takes no notice of EXEC: all lanes read, in no branch)
+          const bf16x8 vs = part_of<F16, true>(v_frag(Vs, dt, f));
+          const bf16x8 pk = only(pr, j, hl == h2), vk = only(vs, j, hl == h2);
           f32x16 t;
 #pragma unroll
           for (int i = 0; i < 16; ++i) t[i] = 0.f;
@@ -919,8 +920,7 @@ __global__ void __launch_bounds__(NT, 2) attn_paged_step(PagedArgs p) {
           for (int jj = 0; jj < 32; ++jj) {
             const int j = jj & 7, g2 = jj >> 3;
             const int key = key0 + 4 * g2 + (j & 3) + 16 * (j >> 2);
-            const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
-            const bf16x8 pk = g == g2 ? only(pf, j) : z, vk = g == g2 ? only(vs, j) : z;
+            const bf16x8 pk = only(pf, j, g == g2), vk = only(vs, j, g == g2);
             const f32x4 x = mfma16x16x32<F16>(vk, pk, f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
             for (int i = 0; i < 4; ++i) sum[i] = key < limit[rb] ? sum[i] + x[i] : sum[i];

@@ -159,3 +159,31 @@ def test_results_do_not_depend_on_what_is_hidden(nat, kind, pages, seqs, heads, 
         assert torch.equal(lse[:, hidden], wlse[:, hidden]), change.__name__
         if change is large:
             assert not torch.equal(got[~hidden], want[~hidden])
+
+
+@pytest.mark.parametrize("kind,pages", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16),
+                                        (torch.bfloat16, E4M3), (torch.float16, torch.int8)], ids=str)
+@pytest.mark.parametrize("new,heads,first", [(100, 1, 256), (100, 3, 256), (8, 2, 288), (300, 1, 256)])
+def test_a_special_value_anywhere_in_a_tile_stays_hidden(nat, kind, pages, new, heads, first):
+    """A NaN in every dim, or an infinity in one, of each key of a tile in turn: the rows that do not see the key keep their
+    bits, whatever else of the tile they see."""
+    total = first + 100 if new > 8 else first + 8
+    q = _randn(new, heads, 64, seed=2, dtype=kind)
+
+    def run(key=None, dim=None):
+        def spoil(batch, k, v):
+            if key is not None:
+                v[key, :, slice(None) if dim is None else dim] = math.nan if dim is None else math.inf
+
+        s = Scene([(new, total)], 1, 16, pages, seed=1)
+        s.fill(1, kind, change=spoil)
+        return _attend(nat, s, q, 1, False)[0]
+
+    want = run()
+    limit = torch.tensor(ref.limits(new, total, 1), device="cuda")
+    for key in range(first, min(first + 64, total)):
+        hidden = limit <= key
+        for dim in (None, (7 * key) % 64):
+            got = run(key, dim)
+            assert torch.equal(got[hidden], want[hidden]), (key - first, dim)
+            assert not torch.isfinite(got[~hidden].float()).all(-1).any() or not (~hidden).any()
