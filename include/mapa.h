@@ -549,7 +549,8 @@ int mapa_kv_cache_read(const mapa_kv_cache* c, const mapa_kv_batch* b, const int
  * sees itself and the earlier ones).  A query that sees nothing (more new tokens than cached ones) gets o = 0,
  * lse = -inf.  A query's output depends on the keys and values it sees alone, to the last bit, whatever the hidden rows
  * hold.  A row whose scores are all -inf is NaN, and so is its lse.  Scores are fp32: beyond 2^24 in magnitude (scale q.k)
- * they are no finer than one, and past 2^28 a row's sum may vanish or overflow.
+ * they are no finer than one, and past 2^28 a row's sum may vanish or overflow.  Probabilities are multiplied in q's type:
+ * one that it rounds to zero (fp16: under 2^-32 of the row's largest) makes NaN of an infinite value that the row sees.
  * lse (optional): [heads][new_rows] natural log, as mapa_attn_merge takes it.
  * scale: softmax scale on q.k (0 = 1/8).  workspace (mapa_attention_paged_workspace_bytes, any contents, not shared
  * with a call that may run at the same time): fp32 partials of the key ranges that are computed apart when there are
